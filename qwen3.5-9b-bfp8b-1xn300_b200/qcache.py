@@ -15,7 +15,8 @@ import re
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libqcache.so")
-HEADERS = [os.path.join(HERE, "..", "include", h) for h in ("qcache.h", "qbfp8.h", "qsample.h")]
+HEADERS = [os.path.join(HERE, "..", "include", h) for h in ("qcache.h", "qbfp8.h", "qsample.h", "qrope.h",
+                                                               "qkv8.h")]
 
 QC_OK, QC_ERR_ARG, QC_ERR_OOM, QC_ERR_CUDA, QC_ERR_TIMEOUT, QC_ERR_BOUNDS, QC_ERR_NODEVICE = range(7)
 QC_FLAG_REFERENCE_MATH = 1
@@ -44,6 +45,58 @@ class Config(C.Structure):
         ("max_batch", C.c_int32),
         ("max_snapshots", C.c_int32),
         ("flags", C.c_int32),
+    ]
+
+
+class RopeConfig(C.Structure):
+    _fields_ = [
+        ("rot_dim", C.c_int32),
+        ("layout", C.c_int32),
+        ("scaling", C.c_int32),
+        ("orig_ctx", C.c_int32),
+        ("base", C.c_double),
+        ("factor", C.c_double),
+        ("beta_fast", C.c_double),
+        ("beta_slow", C.c_double),
+        ("mscale", C.c_double),
+    ]
+
+
+class RopeFrequencies(C.Structure):
+    _fields_ = [
+        ("rot_dim", C.c_int32),
+        ("layout", C.c_int32),
+        ("mscale", C.c_double),
+        ("inv_freq", C.c_double * 128),
+    ]
+
+
+class RopePart(C.Structure):
+    """One group of heads of every row (qc_rope_part): RopePart(x_ptr, out_ptr,
+    n_heads, x_ld, x_head, out_ld, out_head, norm_ptr=0), strides in elements."""
+    _fields_ = [
+        ("x", C.c_void_p),
+        ("out", C.c_void_p),
+        ("norm_w", C.c_void_p),
+        ("x_ld", C.c_int64),
+        ("x_head", C.c_int64),
+        ("out_ld", C.c_int64),
+        ("out_head", C.c_int64),
+        ("n_heads", C.c_int32),
+        ("reserved", C.c_int32),
+    ]
+
+    def __init__(self, x_ptr, out_ptr, n_heads, x_ld, x_head, out_ld, out_head, norm_ptr=0):
+        super().__init__(x_ptr, out_ptr, norm_ptr, x_ld, x_head, out_ld, out_head, n_heads, 0)
+
+
+class Kv8Desc(C.Structure):
+    _fields_ = [
+        ("pool", C.c_void_p),
+        ("n_pages", C.c_int32),
+        ("n_kv_heads", C.c_int32),
+        ("head_dim", C.c_int32),
+        ("reserved", C.c_int32),
     ]
 
 
@@ -127,6 +180,18 @@ def lib() -> C.CDLL:
         "qc_bfp8_gemv_split": (C.c_int, [P, P, I32, I32, P, P, P]),
         "qc_bfp8_check": (C.c_int, [P]),
         "qc_sample": (C.c_int, [P, C.c_int64, I32, I32, C.c_float, C.c_float, P, P, P]),
+        "qc_rope_init": (C.c_int, [C.POINTER(RopeConfig), C.POINTER(RopeFrequencies)]),
+        "qc_rope_apply": (C.c_int, [C.POINTER(RopeFrequencies), I32, C.c_float, P, I32,
+                                    C.POINTER(RopePart), I32, P]),
+        "qc_kv8_page_bytes": (C.c_int64, [I32, I32]),
+        "qc_kv8_write": (C.c_int, [C.POINTER(Kv8Desc), P, I32, P, P, I32, I32, P, C.c_int64, P,
+                                   C.c_int64, P]),
+        "qc_kv8_read": (C.c_int, [C.POINTER(Kv8Desc), P, I32, P, P, I32, I32, P, C.c_int64, P,
+                                  C.c_int64, P]),
+        "qc_kv8_attn_workspace_bytes": (C.c_int64, [C.POINTER(Kv8Desc), I32, I32]),
+        "qc_kv8_attn_decode": (C.c_int, [C.POINTER(Kv8Desc), P, I32, P, I32, I32, P, C.c_int64,
+                                         C.c_int64, P, C.c_float, P, C.c_int64, P, C.c_int64, P]),
+        "qc_kv8_check": (C.c_int, [P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)
@@ -431,3 +496,67 @@ def sample(logits_ptr, ld, vocab, batch, temperature, top_p, uniform_ptr, tokens
                      stream)
     if rc:
         raise QCacheError(rc, L.qc_last_error(None).decode())
+
+
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = 0, 1, 2, 3
+
+
+def _ck_thread(rc):
+    if rc:
+        raise QCacheError(rc, lib().qc_last_error(None).decode())
+
+
+class Rope:
+    """Rotary frequencies and their application (include/qrope.h)."""
+
+    def __init__(self, rot_dim, layout=ROPE_HALF, base=1e7, scaling=ROPE_PLAIN, factor=1.0,
+                 orig_ctx=0, beta_fast=0.0, beta_slow=0.0, mscale=0.0):
+        cfg = RopeConfig(rot_dim, layout, scaling, orig_ctx, base, factor, beta_fast, beta_slow,
+                         mscale)
+        self.freq = RopeFrequencies()
+        _ck_thread(lib().qc_rope_init(C.byref(cfg), C.byref(self.freq)))
+
+    def apply(self, head_dim, pos_ptr, n_rows, parts, eps=1e-6, stream=0):
+        """qc_rope_apply over a list of RopePart."""
+        arr = (RopePart * len(parts))(*parts)
+        _ck_thread(lib().qc_rope_apply(C.byref(self.freq), head_dim, eps, pos_ptr, n_rows, arr,
+                                       len(parts), stream))
+
+
+def kv8_page_bytes(n_kv_heads, head_dim) -> int:
+    return lib().qc_kv8_page_bytes(n_kv_heads, head_dim)
+
+
+def kv8_check(stream=0):
+    """qc_kv8_check: raise the first error that the 8-bit cache's kernels have
+    recorded on the current device since the last check (and clear it)."""
+    _ck_thread(lib().qc_kv8_check(stream))
+
+
+class Kv8Cache:
+    """An 8-bit paged KV pool in the caller's device memory (include/qkv8.h)."""
+
+    def __init__(self, pool_ptr, n_pages, n_kv_heads, head_dim):
+        self.desc = Kv8Desc(pool_ptr, n_pages, n_kv_heads, head_dim, 0)
+
+    def write(self, table_ptr, pt_stride, pos_ptr, row_start_ptr, n, n_rows, k_ptr, k_ld, v_ptr,
+              v_ld, stream=0):
+        """qc_kv8_write; row_start_ptr 0: one row per sequence."""
+        _ck_thread(lib().qc_kv8_write(C.byref(self.desc), table_ptr, pt_stride, pos_ptr,
+                                      row_start_ptr, n, n_rows, k_ptr, k_ld, v_ptr, v_ld, stream))
+
+    def read(self, table_ptr, pt_stride, pos_ptr, row_start_ptr, n, n_rows, k_ptr, k_ld, v_ptr,
+             v_ld, stream=0):
+        _ck_thread(lib().qc_kv8_read(C.byref(self.desc), table_ptr, pt_stride, pos_ptr,
+                                     row_start_ptr, n, n_rows, k_ptr, k_ld, v_ptr, v_ld, stream))
+
+    def attn_workspace_bytes(self, n, n_head) -> int:
+        return lib().qc_kv8_attn_workspace_bytes(C.byref(self.desc), n, n_head)
+
+    def attn_decode(self, table_ptr, pt_stride, len_ptr, n, n_head, q_ptr, q_ld, q_head, gate_ptr,
+                    scale, out_ptr, out_ld, workspace_ptr, workspace_bytes, stream=0):
+        """qc_kv8_attn_decode; gate_ptr 0: no output gate."""
+        _ck_thread(lib().qc_kv8_attn_decode(C.byref(self.desc), table_ptr, pt_stride, len_ptr, n,
+                                            n_head, q_ptr, q_ld, q_head, gate_ptr, scale, out_ptr,
+                                            out_ld, workspace_ptr, workspace_bytes, stream))
