@@ -15,7 +15,14 @@ at its largest over the tokens, and N = len / 16 blocks:
   - f32 sums of D products of q and k: (D + 8) 2^-23 S on a score, so as much
     on the weight's exponent; the exponential and its argument 8 * 2^-23 (1 + S);
   - f32 sums over N + 16 blocks' weights and products: (N + 16) 2^-23 A, twice
-    (numerator and denominator).
+    (numerator and denominator);
+  - f16 ends at 2^-24: a weight w_j = 2^(x_j - r) sv_j (sv_j the block's V scale)
+    is off by up to 2^-25 however small it is.  The largest w_j was at least 2^7
+    when r was last set, so 2^(r - m) / l <= 2^-7 max_j(p_j sv_j), and the len
+    weights' errors on codes of at most 127 come to len 2^-25 127 2^-7
+    max_j(p_j sv_j) <= len 2^-31 max_j(p_j u_j), u_j the largest |v| of token j's
+    block (127 sv <= 2 u).  It matters only for a dim in which the tokens with
+    the weight have code 0.
 """
 import math
 
@@ -352,7 +359,9 @@ def check_attention(got, q, gate, kvs, scale):
         s = (qi.abs() @ kk.abs() * abs(scale)).amax(-1, keepdim=True)
         n = len(k) / 16
         f = (0 if group <= 4 else 2.0 ** -11) + 4 * 2.0 ** -22 + (dim + 8) * 2.0 ** -23 * s + 8 * 2.0 ** -23 * (1 + s)
-        tol = a * (f + 2 * (n + 16) * 2.0 ** -23)
+        u = torch.cat([b.abs().amax((1, 2), keepdim=True).expand(-1, b.shape[1], 1) for b in vv.split(16, 1)], 1)
+        end = len(k) * 2.0 ** -31 * (p * u.transpose(1, 2)).amax(-1, keepdim=True)
+        tol = a * (f + 2 * (n + 16) * 2.0 ** -23) + end
         if gate is not None:
             w = torch.sigmoid(gate[i].double().unflatten(0, (kv, group)))
             y, tol = y * w, tol * w + y.abs() * w * 8 * 2.0 ** -24
