@@ -32,6 +32,7 @@ extern "C" {
 
 #define QC_ROPE_MAX_DIM   256     /* largest head_dim and rot_dim */
 #define QC_ROPE_MAX_PARTS 4
+#define QC_ROPE_MAX_HEADS 16384 /* heads of a part */
 
 /* pair layouts */
 #define QC_ROPE_HALF        0
@@ -86,7 +87,7 @@ typedef struct qc_rope_part {
   uint16_t* out;         /* bf16, device */
   const float* norm_w;   /* [head_dim] f32, device; NULL: no norm */
   int64_t x_ld, x_head, out_ld, out_head;
-  int32_t n_heads;
+  int32_t n_heads;       /* 1 .. QC_ROPE_MAX_HEADS */
   int32_t reserved;      /* 0 */
 } qc_rope_part;
 

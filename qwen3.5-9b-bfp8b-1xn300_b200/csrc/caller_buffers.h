@@ -1,5 +1,6 @@
-// caller_buffers.h — checks shared by the calls that work on the caller's own
-// device buffers (rope.cu, kv8.cu): every one refuses before it launches.
+// caller_buffers.h — what the calls that work on the caller's own device buffers
+// share (rope.cu, kv8.cu): the checks, every one of which refuses before anything
+// is launched, and the launch.
 #pragma once
 
 #include <cstdarg>
@@ -44,6 +45,24 @@ inline int check_device_pointer(const char* call, const char* name, const void* 
     return refuse(QC_ERR_ARG, "%s: %s is on device %d, the current one is %d", call, name,
                   at.device, dev);
   return QC_OK;
+}
+
+// Launch as a programmatic dependent of the kernel before: it may start early and
+// waits (griddepcontrol.wait) before it reads or writes memory.
+template <typename... A>
+cudaError_t launch_dependent(void (*k)(A...), dim3 grid, int threads, size_t smem, cudaStream_t s,
+                             const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k, args...);
 }
 
 }  // namespace qc

@@ -679,22 +679,6 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnArgs a) {
   }
 }
 
-template <typename... A>
-cudaError_t launch_dependent(void (*k)(A...), dim3 grid, int threads, size_t smem, cudaStream_t s,
-                             const A&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads, 1, 1);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k, args...);
-}
-
 // Workspace: owners of MAX_WARPS warps, then their records.
 int64_t owner_bytes() { return int64_t(MAX_WARPS) * sizeof(int4); }
 int64_t record_bytes(int32_t group, int32_t dim) { return int64_t(group) * (dim + 4) * sizeof(float); }

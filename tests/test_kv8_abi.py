@@ -85,6 +85,7 @@ def test_rope_apply_refuses(qcache):
     call("eps", eps=-1.0)
     call("eps", eps=math.nan)
     call("n_heads", n_heads=0)
+    call("n_heads", n_heads=16385)
     for s in ("x_ld", "x_head", "out_ld", "out_head"):
         call("multiples of 8", **{s: 1020})
     for s in ("x_ptr", "out_ptr", "norm_ptr"):
