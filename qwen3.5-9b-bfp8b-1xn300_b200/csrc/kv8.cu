@@ -32,24 +32,8 @@ __host__ __device__ constexpr int block_bytes(int dim) { return HEAD_BYTES + 2 *
 // First error of these kernels on this device since the last qc_kv8_check.
 __device__ int g_kv8_error;
 
-struct Kv8RowsArgs {
-  uint8_t* pool;
-  const int32_t *table, *pos, *start;  // start null: one row each
-  uint16_t *k, *v;
-  int64_t k_ld, v_ld;
-  int32_t n_pages, pt_stride, kv_heads, n, rows;
-};
-
 __device__ __forceinline__ int64_t blocks_touched(int64_t pos, int64_t cnt) {
   return cnt > 0 ? (pos + cnt - 1) / BT - pos / BT + 1 : 0;
-}
-
-// bf16 bits as the value that is quantised: NaN is 0, what 127 * 2^120 does not
-// reach saturates there.
-__device__ __forceinline__ float storable(uint16_t b) {
-  const float x = bf2f(b);
-  const float most = 0x1.FCp+126f;  // 127 * 2^120
-  return x != x ? 0.0f : fminf(fmaxf(x, -most), most);
 }
 
 // The smallest power of two s with amax <= 127 s, at least 2^-126.  With amax =
@@ -61,152 +45,325 @@ __device__ __forceinline__ float pow2_scale(float amax) {
   return __uint_as_float(uint32_t(e + 127) << 23);
 }
 
-__device__ __forceinline__ uint32_t code_of(float x, float inv) {
-  return uint32_t(__float2int_rn(fminf(fmaxf(x * inv, -127.0f), 127.0f)) + 128);
+struct Kv8RowsArgs {
+  uint8_t* pool;
+  const int32_t *table, *pos, *start;  // start null: one row each
+  uint16_t *k, *v;
+  int64_t k_ld, v_ld;
+  int32_t n_pages, pt_stride, kv_heads, n, rows;
+};
+
+// ------------------------------------------------- blocks of many sequences
+
+// Blocks of the sequences before this thread's run of them, and of all.  The
+// sequences are dealt to the CTA's threads in runs, whose sums are scanned.
+template <int WARPS, typename Count>
+__device__ __forceinline__ void scan_blocks(int n, Count count, int64_t* sums, int64_t& before,
+                                            int64_t& mine, int64_t& total) {
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const int run = (n + 32 * WARPS - 1) / (32 * WARPS);
+  mine = 0;
+  for (int i = tid * run; i < min((tid + 1) * run, n); ++i) mine += count(i);
+  before = mine;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const int64_t x = __shfl_up_sync(FULL_MASK, before, m);
+    if (lane >= m) before += x;
+  }
+  if (lane == 31) sums[w] = before;
+  __syncthreads();
+  total = 0;
+  before -= mine;
+#pragma unroll
+  for (int x = 0; x < WARPS; ++x) {
+    if (x < w) before += sums[x];
+    total += sums[x];
+  }
 }
 
-// One CTA of D threads per (touched block, kv head); warp i holds dims 32 i ..
-// 32 i + 31 and each thread the 16 bytes of K and of V that it also writes.
+// The sequence of this thread's run that holds block b, and the block's number
+// in it; b lies in [before, before + mine).
+template <int WARPS, typename Count>
+__device__ __forceinline__ int find_block(int n, Count count, int64_t before, int64_t b,
+                                          int64_t& in) {
+  int i = threadIdx.x * ((n + 32 * WARPS - 1) / (32 * WARPS));
+  for (int64_t nb = count(i); b >= before + nb; nb = count(++i)) before += nb;
+  in = b - before;
+  return i;
+}
+
+// ------------------------------------------------------------ write and read
+
+constexpr int TW = 4;  // warps per CTA
+
+// Codes of four values: x / scale lands in the low mantissa bits of 1.5 * 2^23 +
+// 128, rounded once, to nearest even (the product alone is exact).
+__device__ __forceinline__ uint32_t codes4(float a, float b, float c, float d, float inv) {
+  constexpr float MAGIC = 12582912.0f + 128.0f;
+  const uint32_t x = __float_as_uint(fmaf(a, inv, MAGIC)), y = __float_as_uint(fmaf(b, inv, MAGIC));
+  const uint32_t z = __float_as_uint(fmaf(c, inv, MAGIC)), w = __float_as_uint(fmaf(d, inv, MAGIC));
+  return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
+}
+__device__ __forceinline__ float value_of(uint32_t word, int byte, float scale) {
+  // byte u under 0x4b000000 is 2^23 + u
+  const uint32_t u = __byte_perm(word, 0x4b000000u, 0x7440 + byte);
+  return (__uint_as_float(u) - 8388736.0f) * scale;
+}
+// Older codes under a grown scale (ratio = old / new, a power of two below 1).
+__device__ __forceinline__ uint32_t recode4(uint32_t word, float ratio) {
+  return codes4(value_of(word, 0, 1.0f), value_of(word, 1, 1.0f), value_of(word, 2, 1.0f),
+                value_of(word, 3, 1.0f), ratio);
+}
+__device__ __forceinline__ uint32_t absmax2(uint32_t m, uint32_t pair) {
+  return __vmaxu2(m, pair & 0x7fff7fffu);  // bf16 magnitudes order as their bits
+}
+// NaN to 0, magnitudes beyond 127 * 2^120 to that, both halves of a word.
+constexpr uint32_t MOST_BITS = 0x7efe;
+__device__ __forceinline__ uint32_t storable2(uint32_t pair) {
+  const uint32_t mag = pair & 0x7fff7fffu;
+  return (__vminu2(mag, MOST_BITS * 0x10001u) | (pair & 0x80008000u)) & ~__vcmpgtu2(mag, 0x7f807f80u);
+}
+
+// A tile is the K or the V of one block and head, 16 tokens x D, held by D / 8
+// lanes: lane ll has dims 8 ll .. 8 ll + 7 of every token, a 16-byte load or
+// store per token, all in flight at once.  Rows and codes meet in 16 D bytes of
+// shared memory per tile, which stand in the pool's order (16-byte chunks, D / 32
+// groups of 32) with each group's chunks swapped about by its number, so that
+// neither side's accesses share banks.  Bound by memory.
+#ifndef OCC_
+#define OCC_ 4
+#endif
 template <int D, bool WRITE>
-__global__ void __launch_bounds__(D) kv8_rows_kernel(const Kv8RowsArgs a) {
-  __shared__ int64_t found[2];
-  __shared__ int64_t sums[D];
-  __shared__ float amax_s[2][D / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int head = blockIdx.y;
+__global__ void __launch_bounds__(32 * TW, WRITE ? OCC_ : 1) kv8_rows_kernel(const Kv8RowsArgs a) {
+  constexpr int LPT = D / 8, TILES = 32 / LPT;  // lanes per tile, tiles per warp
+  __shared__ __align__(128) uint8_t stage[TW][TILES * BT * D];
+  __shared__ uint4 older[WRITE ? TW : 1][256];  // a partly new block's chunks before, each lane's own
+  __shared__ int64_t sums[TW];
+  __shared__ struct { int64_t nth; int32_t seq, pos, row, cnt; } at[TW / 2 * TILES];
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const int ll = lane % LPT, tile = lane / LPT;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  // which sequence and which of its blocks this CTA is: the blocks of all
-  // sequences, counted in order
+  // Two warps take the K and the V of the same TILES (block, head) pairs, which
+  // count the heads of a block, then the blocks.
+  constexpr int PAIRS = TW / 2 * TILES;  // of a CTA
+  const int sel = w & 1, slot = (w >> 1) * TILES + tile;
+  const uint32_t heads = a.kv_heads, u0 = blockIdx.x * PAIRS, u = u0 + slot, ub = u / heads;
+  const int head = int(u - ub * heads);
+  int seq;
+  int64_t nth = 0;  // of the sequence's touched blocks
+  int64_t first = 0, row0 = 0, cnt = 1;  // its first position, row and number of rows
   if (a.start) {
-    int64_t base = 0;
-    if (tid == 0) found[0] = -1;
-    __syncthreads();
-    for (int i0 = 0; i0 < a.n; i0 += D) {
-      const int i = i0 + tid;
-      int64_t nb = 0;
-      if (i < a.n) {
-        const int64_t cnt = int64_t(a.start[i + 1]) - a.start[i];
-        nb = a.pos[i] < 0 ? 0 : blocks_touched(a.pos[i], cnt);
-        if (a.pos[i] < 0 && cnt > 0) record_error(&g_kv8_error, QC_ERR_BOUNDS);
+    const auto count = [&](int i) -> int64_t {
+      const int64_t cnt = int64_t(a.start[i + 1]) - a.start[i];
+      if (cnt > 0 && a.pos[i] < 0) record_error(&g_kv8_error, QC_ERR_BOUNDS);
+      return a.pos[i] < 0 ? 0 : blocks_touched(a.pos[i], cnt);
+    };
+    if (tid < PAIRS) at[tid].seq = -1;
+    int64_t before, mine, total;
+    scan_blocks<TW>(a.n, count, sums, before, mine, total);
+    if (mine > 0) {
+      uint32_t b = u0 / heads, left = (b + 1) * heads - u0;
+      for (int x = 0; x < PAIRS; ++x) {
+        if (b >= before && b < before + mine) {
+          int64_t nth;
+          const int i = find_block<TW>(a.n, count, before, b, nth);
+          at[x] = {nth, i, a.pos[i], a.start[i], int32_t(min(int64_t(a.start[i + 1]) - a.start[i], int64_t(INT32_MAX)))};
+        }
+        if (--left == 0) {
+          ++b;
+          left = heads;
+        }
       }
-      sums[tid] = nb;
-      __syncthreads();
-      for (int m = 1; m < D; m <<= 1) {
-        const int64_t add = tid >= m ? sums[tid - m] : 0;
-        __syncthreads();
-        sums[tid] += add;
-        __syncthreads();
-      }
-      const int64_t begin = base + sums[tid] - nb, b = blockIdx.x;
-      if (b >= begin && b < begin + nb) {
-        found[0] = i;
-        found[1] = b - begin;
-      }
-      base += sums[D - 1];
-      __syncthreads();
     }
-    // rows that overlap or leave the input can ask for more blocks than there are CTAs
-    if (tid == 0 && base > int64_t(gridDim.x)) record_error(&g_kv8_error, QC_ERR_BOUNDS);
-  } else if (tid == 0) {
-    found[0] = blockIdx.x;
-    found[1] = 0;
-    if (a.pos[blockIdx.x] < 0) {
+    // rows that overlap or leave the input can ask for more blocks than the launch has
+    if (blockIdx.x == 0 && tid == 0 && total * a.kv_heads > int64_t(gridDim.x) * PAIRS)
       record_error(&g_kv8_error, QC_ERR_BOUNDS);
-      found[0] = -1;
+    __syncthreads();
+    seq = at[slot].seq;
+    nth = at[slot].nth;
+    first = at[slot].pos;
+    row0 = at[slot].row;
+    cnt = at[slot].cnt;
+  } else {
+    seq = ub < uint32_t(a.n) ? int(ub) : -1;
+    row0 = seq;
+    if (seq >= 0) first = a.pos[seq];
+    if (first < 0) {
+      record_error(&g_kv8_error, QC_ERR_BOUNDS);
+      seq = -1;
     }
   }
-  __syncthreads();
-  const int seq = int(found[0]);
-  if (seq < 0) return;
-  const int64_t first = a.pos[seq];
-  const int64_t row0 = a.start ? a.start[seq] : seq;
-  const int64_t cnt = a.start ? a.start[seq + 1] - row0 : 1;
-  const int64_t begin = (first / BT + found[1]) * BT;          // first position of the block
-  const int lo = first > begin ? int(first - begin) : 0;       // new rows of the block: [lo, hi)
-  const int hi = int(min(first + cnt - begin, int64_t(BT)));
-  const int64_t row_of = row0 + begin - first;                 // input row of slot 0
-  const int64_t pg = begin / QC_PAGE;
-  const int32_t page = pg < a.pt_stride ? a.table[int64_t(seq) * a.pt_stride + pg] : -1;
-  if (page < 0 || page >= a.n_pages || row_of + lo < 0 || row_of + hi > a.rows) {
-    if (tid == 0) record_error(&g_kv8_error, QC_ERR_BOUNDS);
-    return;
-  }
-  uint8_t* block = a.pool + ((int64_t(page) * a.kv_heads + head) * PAGE_BLOCKS + begin % QC_PAGE / BT) *
-                                block_bytes(D);
-  uint4* kc = reinterpret_cast<uint4*>(block + HEAD_BYTES) + tid;
-  uint4* vc = kc + D;  // 16 * D bytes further
-  const int g = lane >> 2, t = lane & 3;
-  const int rho = 4 * (g >> 1) + (g & 1);
-  // slot and dim of byte e of this thread's 16 K bytes and of its 16 V bytes
-  auto k_slot = [&](int e) { return rho + 2 * ((e >> 2) & 1); };
-  auto k_dim = [&](int e) { return 32 * warp + 16 * (e >> 3) + 4 * t + (e & 3); };
-  auto v_slot = [&](int e) { return 4 * t + (e & 3); };
-  auto v_dim = [&](int e) { return 32 * warp + 16 * (e >> 3) + 8 * ((e >> 2) & 1) + g; };
 
-  if (!WRITE) {
-    const float2 sc = *reinterpret_cast<const float2*>(block);
-    const uint4 kw = *kc, vw = *vc;
-    const uint8_t* kb = reinterpret_cast<const uint8_t*>(&kw);
-    const uint8_t* vb = reinterpret_cast<const uint8_t*>(&vw);
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      if (k_slot(e) >= lo && k_slot(e) < hi)
-        a.k[(row_of + k_slot(e)) * a.k_ld + head * D + k_dim(e)] = f2bf(float(int(kb[e]) - 128) * sc.x);
-      if (v_slot(e) >= lo && v_slot(e) < hi)
-        a.v[(row_of + v_slot(e)) * a.v_ld + head * D + v_dim(e)] = f2bf(float(int(vb[e]) - 128) * sc.y);
+  int lo = 0, hi = 0;  // the block's tokens that are rows of this call: [lo, hi)
+  int64_t row = 0;     // input row of token 0
+  uint8_t* block = nullptr;
+  if (seq >= 0) {
+    const int64_t begin = (first / BT + nth) * BT;
+    lo = first > begin ? int(first - begin) : 0;
+    hi = int(min(first + cnt - begin, int64_t(BT)));
+    row = row0 + begin - first;
+    const int64_t pg = begin / QC_PAGE;
+    const int32_t page = pg < a.pt_stride ? a.table[int64_t(seq) * a.pt_stride + pg] : -1;
+    if (page < 0 || page >= a.n_pages || row + lo < 0 || row + hi > a.rows) {
+      record_error(&g_kv8_error, QC_ERR_BOUNDS);
+      hi = lo = 0;
+    } else {
+      block = a.pool + ((int64_t(page) * a.kv_heads + head) * PAGE_BLOCKS + begin % QC_PAGE / BT) *
+                           block_bytes(D);
     }
-    return;
   }
+  const int64_t ld = sel ? a.v_ld : a.k_ld;
+  uint16_t* rows = (sel ? a.v : a.k) + row * ld + head * D + 8 * ll;
+  float* scale_at = reinterpret_cast<float*>(block) + sel;
+  uint4* chunks = reinterpret_cast<uint4*>(block + HEAD_BYTES + sel * BT * D);
+  uint8_t* mine = stage[w] + tile * BT * D;
+  // Chunk idx = 4 g + t of group i stands at idx ^ key(i).
+  const auto key = [&](int i) { return (tile * (LPT / 4) + i) & 7; };
+  const auto chunk_at = [&](int i, int idx) { return mine + 512 * i + 16 * (idx ^ key(i)); };
+  // Words of lane ll in that order: K, 4 dims of tokens rho(g) and rho(g) + 2 side by
+  // side, for its runs of dims 8 ll .. + 3 and 8 ll + 4 .. + 7; V, 4 tokens of dim 8 ll + g.
+  const int gi = ll / 4;
+  const auto k_word = [&](int g, int e) {
+    return reinterpret_cast<uint2*>(chunk_at(gi, 4 * g + ((2 * ll + e) & 3)) + 8 * ((ll & 3) >> 1));
+  };
+  const auto v_word = [&](int g, int t) {
+    return reinterpret_cast<uint32_t*>(chunk_at(gi, 4 * g + t) + 4 * (ll & 3));
+  };
 
-  float kx[16], vx[16], ka = 0.0f, va = 0.0f;
+  if (WRITE) {
+    uint4 x[BT];
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    kx[e] = vx[e] = 0.0f;
-    if (k_slot(e) >= lo && k_slot(e) < hi)
-      kx[e] = storable(a.k[(row_of + k_slot(e)) * a.k_ld + head * D + k_dim(e)]);
-    if (v_slot(e) >= lo && v_slot(e) < hi)
-      vx[e] = storable(a.v[(row_of + v_slot(e)) * a.v_ld + head * D + v_dim(e)]);
-    ka = fmaxf(ka, fabsf(kx[e]));
-    va = fmaxf(va, fabsf(vx[e]));
-  }
-  ka = warp_max(ka);
-  va = warp_max(va);
-  if (lane == 0) {
-    amax_s[0][warp] = ka;
-    amax_s[1][warp] = va;
-  }
-  // the block's scales before this call are read before anything is written
-  const float2 old = *reinterpret_cast<const float2*>(block);
-  __syncthreads();
-  for (int w = 0; w < D / 32; ++w) {
-    ka = fmaxf(ka, amax_s[0][w]);
-    va = fmaxf(va, amax_s[1][w]);
-  }
-  float ks = pow2_scale(ka), vs = pow2_scale(va);
-  if (lo > 0) {  // older tokens stay: the scale does not shrink
-    ks = fmaxf(ks, old.x);
-    vs = fmaxf(vs, old.y);
-  }
-  if (tid == 0) *reinterpret_cast<float2*>(block) = make_float2(ks, vs);
-  const float ki = 1.0f / ks, vi = 1.0f / vs;
-  const float kr = old.x / ks, vr = old.y / vs;
-  const bool whole = lo == 0 && hi == BT;
-  uint4 kw = make_uint4(0, 0, 0, 0), vw = kw;
-  if (!whole) {
-    kw = *kc;
-    vw = *vc;
-  }
-  uint8_t* kb = reinterpret_cast<uint8_t*>(&kw);
-  uint8_t* vb = reinterpret_cast<uint8_t*>(&vw);
+    for (int s = 0; s < BT; ++s)
+      x[s] = s >= lo && s < hi ? *reinterpret_cast<const uint4*>(rows + s * ld) : make_uint4(0, 0, 0, 0);
+    const bool part = hi > lo && (lo > 0 || hi < BT);
+    float old_scale = 0.0f;
+    if (part) {
+      old_scale = *scale_at;
 #pragma unroll
-  for (int e = 0; e < 16; ++e) {
-    if (k_slot(e) < lo) kb[e] = uint8_t(code_of(float(int(kb[e]) - 128) * kr, 1.0f));
-    else if (k_slot(e) < hi) kb[e] = uint8_t(code_of(kx[e], ki));
-    if (v_slot(e) < lo) vb[e] = uint8_t(code_of(float(int(vb[e]) - 128) * vr, 1.0f));
-    else if (v_slot(e) < hi) vb[e] = uint8_t(code_of(vx[e], vi));
+      for (int c = 0; c < 8; ++c)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                         smem_u32(&older[w][c * 32 + lane])),
+                     "l"(chunks + c * LPT + ll)
+                     : "memory");
+    }
+    const auto tile_max = [&]() {
+      uint32_t m = 0;
+#pragma unroll
+      for (int s = 0; s < BT; ++s)
+        m = absmax2(absmax2(absmax2(absmax2(m, x[s].x), x[s].y), x[s].z), x[s].w);
+      m = max(m & 0xffffu, m >> 16);
+      for (int d = LPT / 2; d; d >>= 1) m = max(m, __shfl_xor_sync(FULL_MASK, m, d));
+      return m;
+    };
+    uint32_t top = tile_max();
+    if (__any_sync(FULL_MASK, top > MOST_BITS)) {
+#pragma unroll
+      for (int s = 0; s < BT; ++s)
+        x[s] = make_uint4(storable2(x[s].x), storable2(x[s].y), storable2(x[s].z), storable2(x[s].w));
+      top = tile_max();
+    }
+    float scale = pow2_scale(__uint_as_float(top << 16));
+    if (lo > 0) scale = fmaxf(scale, old_scale);  // older tokens stay: the scale does not shrink
+    const float inv = 1.0f / scale, ratio = old_scale / scale;
+    if (sel == 0) {
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        const int rho = 4 * (g >> 1) + (g & 1);
+        const uint4 p = x[rho], q = x[rho + 2];
+        *k_word(g, 0) = make_uint2(codes4(bf_lo(p.x), bf_hi(p.x), bf_lo(p.y), bf_hi(p.y), inv),
+                                   codes4(bf_lo(q.x), bf_hi(q.x), bf_lo(q.y), bf_hi(q.y), inv));
+        *k_word(g, 1) = make_uint2(codes4(bf_lo(p.z), bf_hi(p.z), bf_lo(p.w), bf_hi(p.w), inv),
+                                   codes4(bf_lo(q.z), bf_hi(q.z), bf_lo(q.w), bf_hi(q.w), inv));
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const uint4 p = x[4 * t], q = x[4 * t + 1], r = x[4 * t + 2], z = x[4 * t + 3];
+        *v_word(0, t) = codes4(bf_lo(p.x), bf_lo(q.x), bf_lo(r.x), bf_lo(z.x), inv);
+        *v_word(1, t) = codes4(bf_hi(p.x), bf_hi(q.x), bf_hi(r.x), bf_hi(z.x), inv);
+        *v_word(2, t) = codes4(bf_lo(p.y), bf_lo(q.y), bf_lo(r.y), bf_lo(z.y), inv);
+        *v_word(3, t) = codes4(bf_hi(p.y), bf_hi(q.y), bf_hi(r.y), bf_hi(z.y), inv);
+        *v_word(4, t) = codes4(bf_lo(p.z), bf_lo(q.z), bf_lo(r.z), bf_lo(z.z), inv);
+        *v_word(5, t) = codes4(bf_hi(p.z), bf_hi(q.z), bf_hi(r.z), bf_hi(z.z), inv);
+        *v_word(6, t) = codes4(bf_lo(p.w), bf_lo(q.w), bf_lo(r.w), bf_lo(z.w), inv);
+        *v_word(7, t) = codes4(bf_hi(p.w), bf_hi(q.w), bf_hi(r.w), bf_hi(z.w), inv);
+      }
+    }
+    __syncwarp();
+    if (hi > lo && ll == 0) *scale_at = scale;
+    if (hi > lo && !part) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        chunks[c * LPT + ll] =
+            *reinterpret_cast<const uint4*>(chunk_at((c * LPT + ll) >> 5, (c * LPT + ll) & 31));
+    } else if (hi > lo) {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      // bytes of tokens below lo keep their value, those from hi on their bits;
+      // a word is 4 tokens from 4 t (V) or one token (K: in turn rho(g) and rho(g) + 2)
+      const auto below = [](int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1; };
+      uint32_t kept[2] = {below(lo - 4 * (ll & 3)), 0}, fresh[2] = {below(hi - 4 * (ll & 3)) & ~kept[0], 0};
+      kept[1] = kept[0];
+      fresh[1] = fresh[0];
+#pragma unroll 1
+      for (int c = 0; c < 8; ++c) {
+        const int i = (c * LPT + ll) >> 5, idx = (c * LPT + ll) & 31, g = idx >> 2;
+        if (sel == 0)
+          for (int e = 0; e < 2; ++e) {
+            const int token = 4 * (g >> 1) + (g & 1) + 2 * e;
+            kept[e] = token < lo ? ~0u : 0u;
+            fresh[e] = token < hi ? ~kept[e] : 0u;
+          }
+        const uint4 y = *reinterpret_cast<const uint4*>(chunk_at(i, idx)), old = older[w][c * 32 + lane];
+        const auto merge = [&](uint32_t n, uint32_t was, int e) {
+          if (kept[e] && ratio != 1.0f) was = (recode4(was, ratio) & kept[e]) | (was & ~kept[e]);
+          return (n & fresh[e]) | (was & ~fresh[e]);
+        };
+        chunks[c * LPT + ll] = make_uint4(merge(y.x, old.x, 0), merge(y.y, old.y, 1),
+                                          merge(y.z, old.z, 0), merge(y.w, old.w, 1));
+      }
+    }
+  } else {
+    float scale = 0.0f;
+    if (hi > lo) {
+      scale = *scale_at;
+      uint4 y[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) y[c] = chunks[c * LPT + ll];
+#pragma unroll
+      for (int c = 0; c < 8; ++c)
+        *reinterpret_cast<uint4*>(chunk_at((c * LPT + ll) >> 5, (c * LPT + ll) & 31)) = y[c];
+    }
+    __syncwarp();
+    const auto pair = [&](uint32_t a0, int b0, uint32_t a1, int b1) {
+      const __nv_bfloat162 h = __floats2bfloat162_rn(value_of(a0, b0, scale), value_of(a1, b1, scale));
+      return *reinterpret_cast<const uint32_t*>(&h);
+    };
+    const auto put = [&](int s, uint4 y) {
+      if (s >= lo && s < hi) *reinterpret_cast<uint4*>(rows + s * ld) = y;
+    };
+    if (sel == 0) {
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        const int rho = 4 * (g >> 1) + (g & 1);
+        const uint2 p = *k_word(g, 0), q = *k_word(g, 1);
+        put(rho, make_uint4(pair(p.x, 0, p.x, 1), pair(p.x, 2, p.x, 3), pair(q.x, 0, q.x, 1), pair(q.x, 2, q.x, 3)));
+        put(rho + 2, make_uint4(pair(p.y, 0, p.y, 1), pair(p.y, 2, p.y, 3), pair(q.y, 0, q.y, 1), pair(q.y, 2, q.y, 3)));
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        uint32_t v[8];
+#pragma unroll
+        for (int g = 0; g < 8; ++g) v[g] = *v_word(g, t);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          put(4 * t + e, make_uint4(pair(v[0], e, v[1], e), pair(v[2], e, v[3], e), pair(v[4], e, v[5], e),
+                                    pair(v[6], e, v[7], e)));
+      }
+    }
   }
-  *kc = kw;
-  *vc = vw;
 }
 
 // ---------------------------------------------------------------- attention
@@ -261,7 +418,7 @@ struct AttnSmem {
   alignas(128) uint8_t stage[AW][AS][block_bytes(D)];
   alignas(8) uint64_t full[AW][AS];
   int32_t valid[AW][AS];                                 // tokens of the block; 0: nothing was copied
-  int64_t sums[AW + 1];
+  int64_t sums[AW];
   struct { int64_t unit; int32_t seq; } start[AW];       // first unit of the sequence a warp starts in
 };
 
@@ -327,6 +484,22 @@ struct Cursor {
   }
 };
 
+// Sequences without tokens: a row of zeros and nothing to merge.  Lengths out of
+// range are reported.
+template <int D>
+__device__ __forceinline__ void mark_empty(const Kv8AttnArgs& a) {
+  for (int i = blockIdx.x; i < a.n; i += gridDim.x) {
+    const int32_t len = a.len[i];
+    if (threadIdx.x == 0 && (len < 0 || len > int64_t(a.pt_stride) * QC_PAGE))
+      record_error(&g_kv8_error, QC_ERR_BOUNDS);
+    if (len > 0) continue;
+    for (int d = threadIdx.x * 8; d < a.kv_heads * a.group * D; d += 8 * 32 * AW)
+      *reinterpret_cast<uint4*>(a.out + i * a.out_ld + d) = make_uint4(0, 0, 0, 0);
+    for (int h = threadIdx.x; h < a.kv_heads && a.by_pair; h += 32 * AW)
+      a.owner[i * a.kv_heads + h] = make_int4(0, 0, 0, 0);
+  }
+}
+
 template <int D, bool PAIRED>
 __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
@@ -341,57 +514,21 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  // Blocks before each sequence: thread i sums its run of sequences, the runs
-  // are scanned, and the threads whose run holds a warp's first block say so.
   const int warps = gridDim.x * AW, wid = w * gridDim.x + blockIdx.x;
-  const int run = (a.n + 32 * AW - 1) / (32 * AW);
-  int64_t mine = 0;
-  for (int j = 0; j < run; ++j) {
-    const int i = tid * run + j;
-    if (i < a.n) {
-      const int64_t nb = seq_blocks(a, i);
-      mine += nb;
-      if (blockIdx.x == 0 && (a.len[i] < 0 || a.len[i] > int64_t(a.pt_stride) * QC_PAGE))
-        record_error(&g_kv8_error, QC_ERR_BOUNDS);
-      // a sequence without tokens has a row of zeros and nothing to merge
-      if (nb == 0 && i % int(gridDim.x) == int(blockIdx.x)) {
-        for (int d = 0; d < a.kv_heads * a.group * D; d += 8)
-          *reinterpret_cast<uint4*>(a.out + i * a.out_ld + d) = make_uint4(0, 0, 0, 0);
-        for (int h = 0; h < a.kv_heads && a.by_pair; ++h)
-          a.owner[i * a.kv_heads + h] = make_int4(0, 0, 0, 0);
-      }
-    }
-  }
-  int64_t before = mine;
-#pragma unroll
-  for (int m = 1; m < 32; m <<= 1) {
-    const int64_t x = __shfl_up_sync(FULL_MASK, before, m);
-    if (lane >= m) before += x;
-  }
-  if (lane == 31) sm.sums[w] = before;
-  __syncthreads();
-  int64_t total = 0;
-  before -= mine;
-  for (int x = 0; x < AW; ++x) {
-    if (x < w) before += sm.sums[x];
-    total += sm.sums[x];
-  }
+  if (int(blockIdx.x) < a.n) mark_empty<D>(a);
+  const auto count = [&](int i) { return seq_blocks(a, i); };
+  int64_t before, mine, total;
+  scan_blocks<AW>(a.n, count, sm.sums, before, mine, total);
   total *= a.kv_heads;
-  before *= a.kv_heads;
   const int64_t per = max((total + warps - 1) / warps, int64_t(MIN_BLOCKS));
   for (int x = 0; x < AW; ++x) {
-    const int64_t u = (int64_t(x) * gridDim.x + blockIdx.x) * per;
-    if (u >= before && u < before + mine * a.kv_heads) {
+    const int64_t u = (int64_t(x) * gridDim.x + blockIdx.x) * per;  // warp x's first block
+    if (u >= before * a.kv_heads && u < (before + mine) * a.kv_heads) {
       int64_t at = before;
-      for (int j = 0; j < run; ++j) {
-        const int64_t nb = seq_blocks(a, tid * run + j) * a.kv_heads;
-        if (u < at + nb) {
-          sm.start[x].unit = at;
-          sm.start[x].seq = tid * run + j;
-          break;
-        }
-        at += nb;
-      }
+      int i = tid * ((a.n + 32 * AW - 1) / (32 * AW));
+      for (int64_t nb = count(i); u >= (at + nb) * a.kv_heads; nb = count(++i)) at += nb;
+      sm.start[x].unit = at * a.kv_heads;
+      sm.start[x].seq = i;
     }
   }
   __syncthreads();
@@ -774,17 +911,21 @@ int rows_call(const char* call, bool write, const qc_kv8_cache* c, const int32_t
   a.rows = rows;
   // every touched block holds a new row, and only a sequence's first and last
   // block can hold fewer than 16
-  const int64_t most = std::min<int64_t>(rows, int64_t(rows) / BT + 2 * int64_t(n));
-  const dim3 grid(start ? (unsigned)most : (unsigned)n, (unsigned)c->n_kv_heads);
+  const int64_t blocks =
+      start ? std::min<int64_t>(rows, int64_t(rows) / BT + 2 * int64_t(n)) : int64_t(n);
+  const int64_t per_cta = TW / 2 * (256 / c->head_dim);
+  const int64_t ctas = (blocks * c->n_kv_heads + per_cta - 1) / per_cta;
+  if (ctas * per_cta > INT32_MAX) return refuse(QC_ERR_ARG, "%s: %d rows of %d heads", call, rows, c->n_kv_heads);
+  const dim3 grid((unsigned)ctas);
   cudaStream_t s = (cudaStream_t)stream;
-#define QC_ROWS(D)                                                      \
-  if (write) kv8_rows_kernel<D, true><<<grid, D, 0, s>>>(a);            \
-  else kv8_rows_kernel<D, false><<<grid, D, 0, s>>>(a)
-  if (c->head_dim == 64) { QC_ROWS(64); }
-  else if (c->head_dim == 128) { QC_ROWS(128); }
-  else { QC_ROWS(256); }
+  cudaError_t e;
+#define QC_ROWS(D)                                                                          \
+  e = write ? launch_dependent(kv8_rows_kernel<D, true>, grid, 32 * TW, 0, s, a)            \
+            : launch_dependent(kv8_rows_kernel<D, false>, grid, 32 * TW, 0, s, a)
+  if (c->head_dim == 64) QC_ROWS(64);
+  else if (c->head_dim == 128) QC_ROWS(128);
+  else QC_ROWS(256);
 #undef QC_ROWS
-  const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? QC_OK : refuse(QC_ERR_CUDA, "%s: %s", call, cudaGetErrorString(e));
 }
 
