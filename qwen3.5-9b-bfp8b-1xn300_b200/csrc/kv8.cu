@@ -55,6 +55,11 @@ struct Kv8RowsArgs {
 
 // ------------------------------------------------- blocks of many sequences
 
+// Quotient of two counts, in 32 bits where they fit: the 64-bit division is long.
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+  return ((x | y) >> 32) == 0 ? int64_t(uint32_t(x) / uint32_t(y)) : x / y;
+}
+
 // Blocks of the sequences before this thread's run of them, and of all.  The
 // sequences are dealt to the CTA's threads in runs, whose sums are scanned.
 template <int WARPS, typename Count>
@@ -130,11 +135,8 @@ __device__ __forceinline__ uint32_t storable2(uint32_t pair) {
 // shared memory per tile, which stand in the pool's order (16-byte chunks, D / 32
 // groups of 32) with each group's chunks swapped about by its number, so that
 // neither side's accesses share banks.  Bound by memory.
-#ifndef OCC_
-#define OCC_ 4
-#endif
 template <int D, bool WRITE>
-__global__ void __launch_bounds__(32 * TW, WRITE ? OCC_ : 1) kv8_rows_kernel(const Kv8RowsArgs a) {
+__global__ void __launch_bounds__(32 * TW, WRITE ? 4 : 1) kv8_rows_kernel(const Kv8RowsArgs a) {
   constexpr int LPT = D / 8, TILES = 32 / LPT;  // lanes per tile, tiles per warp
   __shared__ __align__(128) uint8_t stage[TW][TILES * BT * D];
   __shared__ uint4 older[WRITE ? TW : 1][256];  // a partly new block's chunks before, each lane's own
@@ -409,7 +411,6 @@ struct Kv8AttnArgs {
 
 constexpr int AW = 4;                                    // warps per CTA
 constexpr int AS = 3;                                    // blocks in flight per warp
-constexpr int MIN_BLOCKS = 1;                            // blocks of a warp's range at least
 constexpr int MAX_WARPS = 2400;                          // of the grid
 constexpr float LAZY_M = 8.0f, TOP_R = 7.0f, LAZY_R = 15.0f;
 
@@ -419,7 +420,7 @@ struct AttnSmem {
   alignas(8) uint64_t full[AW][AS];
   int32_t valid[AW][AS];                                 // tokens of the block; 0: nothing was copied
   int64_t sums[AW];
-  struct { int64_t unit; int32_t seq; } start[AW];       // first unit of the sequence a warp starts in
+  struct { int64_t unit; int32_t seq, nb, len; } start[AW];  // the sequence a warp starts in, its first unit
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -456,9 +457,12 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
+// Tokens of a sequence, as many as its page-table row can name, and their blocks.
+__device__ __forceinline__ int32_t seq_len(const Kv8AttnArgs& a, int32_t i) {
+  return int32_t(min(int64_t(max(a.len[i], 0)), int64_t(a.pt_stride) * QC_PAGE));
+}
 __device__ __forceinline__ int64_t seq_blocks(const Kv8AttnArgs& a, int32_t i) {
-  const int64_t most = int64_t(a.pt_stride) * QC_PAGE;
-  return (min(max(int64_t(a.len[i]), int64_t(0)), most) + BT - 1) / BT;
+  return (int64_t(seq_len(a, i)) + BT - 1) / BT;
 }
 
 // Where in the order of blocks a warp stands: `unit` counts the blocks of all
@@ -469,7 +473,7 @@ struct Cursor {
 
   __device__ __forceinline__ void enter(const Kv8AttnArgs& a) {
     nb = int32_t(seq_blocks(a, seq));
-    len = int32_t(min(int64_t(a.len[seq]), int64_t(a.pt_stride) * QC_PAGE));
+    len = seq_len(a, seq);
   }
   // To the next pair that has blocks; the caller knows that there is one.
   __device__ __forceinline__ void next_pair(const Kv8AttnArgs& a) {
@@ -485,17 +489,18 @@ struct Cursor {
 };
 
 // Sequences without tokens: a row of zeros and nothing to merge.  Lengths out of
-// range are reported.
+// range are reported.  Dealt to the warps of the grid.
 template <int D>
 __device__ __forceinline__ void mark_empty(const Kv8AttnArgs& a) {
-  for (int i = blockIdx.x; i < a.n; i += gridDim.x) {
+  const int lane = threadIdx.x & 31;
+  for (int i = (threadIdx.x >> 5) * gridDim.x + blockIdx.x; i < a.n; i += gridDim.x * AW) {
     const int32_t len = a.len[i];
-    if (threadIdx.x == 0 && (len < 0 || len > int64_t(a.pt_stride) * QC_PAGE))
+    if (lane == 0 && (len < 0 || len > int64_t(a.pt_stride) * QC_PAGE))
       record_error(&g_kv8_error, QC_ERR_BOUNDS);
     if (len > 0) continue;
-    for (int d = threadIdx.x * 8; d < a.kv_heads * a.group * D; d += 8 * 32 * AW)
+    for (int d = lane * 8; d < a.kv_heads * a.group * D; d += 8 * 32)
       *reinterpret_cast<uint4*>(a.out + i * a.out_ld + d) = make_uint4(0, 0, 0, 0);
-    for (int h = threadIdx.x; h < a.kv_heads && a.by_pair; h += 32 * AW)
+    for (int h = lane; h < a.kv_heads && a.by_pair; h += 32)
       a.owner[i * a.kv_heads + h] = make_int4(0, 0, 0, 0);
   }
 }
@@ -515,33 +520,36 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   const int warps = gridDim.x * AW, wid = w * gridDim.x + blockIdx.x;
-  if (int(blockIdx.x) < a.n) mark_empty<D>(a);
   const auto count = [&](int i) { return seq_blocks(a, i); };
   int64_t before, mine, total;
   scan_blocks<AW>(a.n, count, sm.sums, before, mine, total);
   total *= a.kv_heads;
-  const int64_t per = max((total + warps - 1) / warps, int64_t(MIN_BLOCKS));
+  const int64_t per = max(quotient(total + warps - 1, warps), int64_t(1));
   for (int x = 0; x < AW; ++x) {
     const int64_t u = (int64_t(x) * gridDim.x + blockIdx.x) * per;  // warp x's first block
     if (u >= before * a.kv_heads && u < (before + mine) * a.kv_heads) {
       int64_t at = before;
       int i = tid * ((a.n + 32 * AW - 1) / (32 * AW));
-      for (int64_t nb = count(i); u >= (at + nb) * a.kv_heads; nb = count(++i)) at += nb;
-      sm.start[x].unit = at * a.kv_heads;
-      sm.start[x].seq = i;
+      int64_t nb = count(i);
+      for (; u >= (at + nb) * a.kv_heads; nb = count(++i)) at += nb;
+      sm.start[x] = {at * a.kv_heads, i, int32_t(nb), seq_len(a, i)};
     }
   }
   __syncthreads();
   const int64_t begin = wid * per, end = min(begin + per, total);
   if (lane == 0 && !a.by_pair) a.owner[wid] = make_int4(0, 0, 0, 0);
-  if (begin >= end) return;
+  if (begin >= end) {
+    mark_empty<D>(a);
+    return;
+  }
 
   Cursor c;
   c.unit = begin;
   c.seq = sm.start[w].seq;
-  c.enter(a);
-  c.head = int32_t((begin - sm.start[w].unit) / c.nb);
-  c.blk = int32_t((begin - sm.start[w].unit) % c.nb);
+  c.nb = sm.start[w].nb;
+  c.len = sm.start[w].len;
+  c.head = int32_t(quotient(begin - sm.start[w].unit, c.nb));
+  c.blk = int32_t(begin - sm.start[w].unit - int64_t(c.head) * c.nb);
   Cursor p = c;  // the copies run AS blocks ahead
   int put = 0;
   auto issue = [&]() {  // lane 0: the copy of block p into the next stage
@@ -563,8 +571,22 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
     ++p.unit;
     if (++p.blk == p.nb && p.unit < end) p.next_pair(a);
   };
+  // A pair's queries are loaded before the copies are issued (behind megabytes of
+  // them they would come late), a later pair's while the one before is stored.
+  uint2 raw[KS];
+  const auto load_q = [&]() {
+    const int h = PAIRED ? g & 3 : g;
+    const uint16_t* q = a.q + c.seq * a.q_ld + (int64_t(c.head) * a.group + h) * a.q_head + 4 * t;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      raw[s] = make_uint2(0, 0);
+      if (h < a.group) raw[s] = *reinterpret_cast<const uint2*>(q + 16 * s);
+    }
+  };
+  load_q();
   if (lane == 0)
     for (int s = 0; s < AS; ++s) issue();
+  mark_empty<D>(a);
 
   int get = 0;
   uint32_t parity = 0;
@@ -575,19 +597,10 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
     uint32_t qf[KS][2];
     float qs[2];  // what a column's products count for: scale log2(e) / the power of two in q
     {
-      const int h = PAIRED ? g & 3 : g;
-      uint2 raw[KS];
       uint32_t top = 0;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        raw[s] = make_uint2(0, 0);
-        if (h < a.group)
-          raw[s] = *reinterpret_cast<const uint2*>(
-              a.q + c.seq * a.q_ld + (int64_t(c.head) * a.group + h) * a.q_head + 16 * s + 4 * t);
-        // bf16 magnitudes order as their bits
-        top = max(top, max(max(raw[s].x & 0x7fffu, (raw[s].x >> 16) & 0x7fffu),
-                           max(raw[s].y & 0x7fffu, (raw[s].y >> 16) & 0x7fffu)));
-      }
+      for (int s = 0; s < KS; ++s) top = absmax2(absmax2(top, raw[s].x), raw[s].y);
+      top = max(top & 0xffffu, top >> 16);
       top = max(top, __shfl_xor_sync(FULL_MASK, top, 1));
       top = max(top, __shfl_xor_sync(FULL_MASK, top, 2));
       // up * 2^e: the largest value into [2^13, 2^14), so that values 2^-37 of it stay exact
@@ -692,7 +705,13 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
     }
 
     // ---- the pair's result, or its record
+    const int32_t seq = c.seq, kvh = c.head;
+    const int64_t pair_end = c.unit - c.blk + c.nb;  // its last block's unit, plus one
     const bool done = c.blk == c.nb, whole = done && blk0 == 0;
+    if (done && c.unit < end) {
+      c.next_pair(a);
+      load_q();
+    }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       l[j] += __shfl_xor_sync(FULL_MASK, l[j], 4);
@@ -714,9 +733,9 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
         const float half = 0.5f * (r[j] - m[j]);
         const float f1 = l[j] == 0.0f ? 0.0f : ex2(half) / l[j];
         const float f2 = l[j] == 0.0f ? 0.0f : ex2(r[j] - m[j] - half);
-        const int64_t head = int64_t(c.head) * a.group + h;
-        uint16_t* out = a.out + c.seq * a.out_ld + head * D;
-        const uint16_t* gate = a.gate ? a.gate + c.seq * a.q_ld + head * a.q_head : nullptr;
+        const int64_t head = int64_t(kvh) * a.group + h;
+        uint16_t* out = a.out + seq * a.out_ld + head * D;
+        const uint16_t* gate = a.gate ? a.gate + seq * a.q_ld + head * a.q_head : nullptr;
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -737,12 +756,11 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
     }
     // the range that a pair starts in says what there is to merge
     if (lane == 0 && blk0 == 0 && (!done || a.by_pair)) {
-      const int64_t last = (c.unit - c.blk + c.nb - 1) / per;
-      a.owner[a.by_pair ? c.seq * a.kv_heads + c.head : wid] =
-          make_int4(c.seq, c.head, done ? 0 : int(last) - wid + 1, 2 * wid + (first ? 0 : 1));
+      const int64_t last = quotient(pair_end - 1, per);
+      a.owner[a.by_pair ? seq * a.kv_heads + kvh : wid] =
+          make_int4(seq, kvh, done ? 0 : int(last) - wid + 1, 2 * wid + (first ? 0 : 1));
     }
     first = false;
-    if (done && c.unit < end) c.next_pair(a);
   }
 }
 
@@ -772,6 +790,15 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnArgs a) {
   const int dim = CHUNK * blockIdx.z + tid;
   float gate = 0.0f;
   if (a.gate && tid < CHUNK) gate = bf2f(a.gate[own.x * a.q_ld + head * a.q_head + dim]);
+  const int quad = tid % LANES, slot = tid / LANES;
+  const auto values = [&](int i) {
+    return *reinterpret_cast<const float4*>(rec(i) + 4 + CHUNK * blockIdx.z + 4 * quad);
+  };
+  constexpr int AHEAD = 4;  // of this thread's records, loaded with the heads
+  float4 ahead[AHEAD];
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j)
+    if (slot + j * SLOTS < n) ahead[j] = values(slot + j * SLOTS);
   float m = -INFINITY, r = -INFINITY, l = 0.0f;
   for (int i = tid; i < n; i += 256) {
     const float4 s = *reinterpret_cast<const float4*>(rec(i));
@@ -792,17 +819,19 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnArgs a) {
   }
   l = warp_sum(l == 0.0f || m == M ? l : l * ex2(m - M));
   if (lane == 0) sum_s[w] = l;
-  const int quad = tid % LANES, slot = tid / LANES;
   float4 o = make_float4(0, 0, 0, 0);
-#pragma unroll 4
-  for (int i = slot; i < n; i += SLOTS) {
+  const auto add = [&](int i, const float4& x) {
     const float f = fac[i] == r ? 1.0f : ex2(fac[i] - r);
-    const float4 x = *reinterpret_cast<const float4*>(rec(i) + 4 + CHUNK * blockIdx.z + 4 * quad);
     o.x += x.x * f;
     o.y += x.y * f;
     o.z += x.z * f;
     o.w += x.w * f;
-  }
+  };
+#pragma unroll
+  for (int j = 0; j < AHEAD; ++j)
+    if (slot + j * SLOTS < n) add(slot + j * SLOTS, ahead[j]);
+#pragma unroll 4
+  for (int i = slot + AHEAD * SLOTS; i < n; i += SLOTS) add(i, values(i));
   part[slot][quad] = o;
   __syncthreads();
   if (tid < CHUNK) {
