@@ -410,17 +410,26 @@ struct Kv8AttnArgs {
 };
 
 constexpr int AW = 4;                                    // warps per CTA
-constexpr int AS = 3;                                    // blocks in flight per warp
-constexpr int MAX_WARPS = 2400;                          // of the grid
+// Blocks of a step, what a warp copies and works on at once (8 KB of codes, and
+// the step's fixed part paid once); steps in flight per warp; CTAs per SM.  Of the
+// shapes that fit an SM's shared memory these were the fastest (us): D 256, 64 x
+// 4096: 8 warps of 3 steps 97.7, 12 of 2 98.6, 9 of 3 124; D 128, 33 ragged: steps
+// of 2 blocks 19.3, of 1 block 22.7; D 64, 64 x 8000: 4 blocks in 12 warps 52.7, in
+// 8 warps 55.8, of 2 blocks 54.5, of 1 block 58.
+__host__ __device__ constexpr int step_blocks(int dim) { return 256 / dim; }
+__host__ __device__ constexpr int stages(int dim) { return dim == 64 ? 2 : 3; }
+__host__ __device__ constexpr int ctas_per_sm(int dim) { return dim == 64 ? 3 : 2; }
+constexpr int MAX_WARPS = 1824;                          // of the grid
 constexpr float LAZY_M = 8.0f, TOP_R = 7.0f, LAZY_R = 15.0f;
 
 template <int D>
 struct AttnSmem {
-  alignas(128) uint8_t stage[AW][AS][block_bytes(D)];
+  static constexpr int AS = stages(D);
+  alignas(128) uint8_t stage[AW][AS][step_blocks(D) * block_bytes(D)];
   alignas(8) uint64_t full[AW][AS];
-  int32_t valid[AW][AS];                                 // tokens of the block; 0: nothing was copied
+  int32_t valid[AW][AS];                                 // tokens of the step; 0: nothing was copied
   int64_t sums[AW];
-  struct { int64_t unit; int32_t seq, nb, len; } start[AW];  // the sequence a warp starts in, its first unit
+  struct { int64_t unit; int32_t seq, n, len; } start[AW];  // the sequence a warp starts in, its first unit
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -457,32 +466,35 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-// Tokens of a sequence, as many as its page-table row can name, and their blocks.
+// Tokens of a sequence, as many as its page-table row can name, and their steps.
 __device__ __forceinline__ int32_t seq_len(const Kv8AttnArgs& a, int32_t i) {
   return int32_t(min(int64_t(max(a.len[i], 0)), int64_t(a.pt_stride) * QC_PAGE));
 }
-__device__ __forceinline__ int64_t seq_blocks(const Kv8AttnArgs& a, int32_t i) {
-  return (int64_t(seq_len(a, i)) + BT - 1) / BT;
+template <int D>
+__device__ __forceinline__ int64_t seq_steps(const Kv8AttnArgs& a, int32_t i) {
+  constexpr int ST = BT * step_blocks(D);
+  return (int64_t(seq_len(a, i)) + ST - 1) / ST;
 }
 
-// Where in the order of blocks a warp stands: `unit` counts the blocks of all
-// pairs, `blk` those of the pair (seq, head), which has nb.
+// Where in the order of steps a warp stands: `unit` counts the steps of all
+// pairs, `at` those of the pair (seq, head), which has n.
+template <int D>
 struct Cursor {
   int64_t unit;
-  int32_t seq, head, blk, nb, len;
+  int32_t seq, head, at, n, len;
 
   __device__ __forceinline__ void enter(const Kv8AttnArgs& a) {
-    nb = int32_t(seq_blocks(a, seq));
+    n = int32_t(seq_steps<D>(a, seq));
     len = seq_len(a, seq);
   }
-  // To the next pair that has blocks; the caller knows that there is one.
+  // To the next pair that has tokens; the caller knows that there is one.
   __device__ __forceinline__ void next_pair(const Kv8AttnArgs& a) {
-    blk = 0;
+    at = 0;
     if (++head == a.kv_heads) {
       head = 0;
       do {
         ++seq;
-      } while (seq + 1 < a.n && seq_blocks(a, seq) == 0);
+      } while (seq + 1 < a.n && seq_len(a, seq) == 0);
       enter(a);
     }
   }
@@ -506,10 +518,11 @@ __device__ __forceinline__ void mark_empty(const Kv8AttnArgs& a) {
 }
 
 template <int D, bool PAIRED>
-__global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) {
+__global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const Kv8AttnArgs a) {
   extern __shared__ __align__(128) uint8_t smem_raw[];
   AttnSmem<D>& sm = *reinterpret_cast<AttnSmem<D>*>(smem_raw);
   constexpr int KS = D / 16;  // steps of 16 dims
+  constexpr int AS = stages(D), GB = step_blocks(D);
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   if (lane == 0) {
@@ -520,13 +533,13 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   const int warps = gridDim.x * AW, wid = w * gridDim.x + blockIdx.x;
-  const auto count = [&](int i) { return seq_blocks(a, i); };
+  const auto count = [&](int i) { return seq_steps<D>(a, i); };
   int64_t before, mine, total;
   scan_blocks<AW>(a.n, count, sm.sums, before, mine, total);
   total *= a.kv_heads;
   const int64_t per = max(quotient(total + warps - 1, warps), int64_t(1));
   for (int x = 0; x < AW; ++x) {
-    const int64_t u = (int64_t(x) * gridDim.x + blockIdx.x) * per;  // warp x's first block
+    const int64_t u = (int64_t(x) * gridDim.x + blockIdx.x) * per;  // warp x's first step
     if (u >= before * a.kv_heads && u < (before + mine) * a.kv_heads) {
       int64_t at = before;
       int i = tid * ((a.n + 32 * AW - 1) / (32 * AW));
@@ -543,33 +556,36 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
     return;
   }
 
-  Cursor c;
+  Cursor<D> c;
   c.unit = begin;
   c.seq = sm.start[w].seq;
-  c.nb = sm.start[w].nb;
+  c.n = sm.start[w].n;
   c.len = sm.start[w].len;
-  c.head = int32_t(quotient(begin - sm.start[w].unit, c.nb));
-  c.blk = int32_t(begin - sm.start[w].unit - int64_t(c.head) * c.nb);
-  Cursor p = c;  // the copies run AS blocks ahead
+  c.head = int32_t(quotient(begin - sm.start[w].unit, c.n));
+  c.at = int32_t(begin - sm.start[w].unit - int64_t(c.head) * c.n);
+  Cursor<D> p = c;  // the copies run AS steps ahead
   int put = 0;
-  auto issue = [&]() {  // lane 0: the copy of block p into the next stage
+  auto issue = [&]() {  // lane 0: the copy of step p into the next stage
     if (p.unit >= end) return;
-    const int32_t page = __ldg(a.table + int64_t(p.seq) * a.pt_stride + p.blk / PAGE_BLOCKS);
+    const int32_t block = p.at * GB;
+    const int32_t page = __ldg(a.table + int64_t(p.seq) * a.pt_stride + block / PAGE_BLOCKS);
     const bool ok = page >= 0 && page < a.n_pages;
-    sm.valid[w][put] = ok ? min(p.len - p.blk * BT, BT) : 0;
+    const int32_t tokens = min(p.len - block * BT, GB * BT);
+    sm.valid[w][put] = ok ? tokens : 0;
     if (ok) {
-      mbar_arrive_expect_tx(&sm.full[w][put], block_bytes(D));
+      const uint32_t bytes = (tokens + BT - 1) / BT * block_bytes(D);
+      mbar_arrive_expect_tx(&sm.full[w][put], bytes);
       bulk_g2s(sm.stage[w][put],
-               a.pool + ((int64_t(page) * a.kv_heads + p.head) * PAGE_BLOCKS + p.blk % PAGE_BLOCKS) *
+               a.pool + ((int64_t(page) * a.kv_heads + p.head) * PAGE_BLOCKS + block % PAGE_BLOCKS) *
                             block_bytes(D),
-               block_bytes(D), &sm.full[w][put]);
+               bytes, &sm.full[w][put]);
     } else {
       record_error(&g_kv8_error, QC_ERR_BOUNDS);
       mbar_arrive(&sm.full[w][put]);
     }
     put = put + 1 == AS ? 0 : put + 1;
     ++p.unit;
-    if (++p.blk == p.nb && p.unit < end) p.next_pair(a);
+    if (++p.at == p.n && p.unit < end) p.next_pair(a);
   };
   // A pair's queries are loaded before the copies are issued (behind megabytes of
   // them they would come late), a later pair's while the one before is stored.
@@ -593,7 +609,7 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
   bool first = true;
   while (c.unit < end) {
     // ---- the pair's queries, as operand columns: column n is head n (PAIRED: n % 4)
-    const int32_t blk0 = c.blk;
+    const int32_t from = c.at;
     uint32_t qf[KS][2];
     float qs[2];  // what a column's products count for: scale log2(e) / the power of two in q
     {
@@ -622,9 +638,9 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
 #pragma unroll
     for (int s = 0; s < KS; ++s) o[s][0] = o[s][1] = o[s][2] = o[s][3] = 0.0f;
 
-    const int32_t stop = int32_t(min(int64_t(c.nb), c.blk + (end - c.unit)));
-    for (; c.blk < stop; ++c.blk, ++c.unit) {
-      if (!mbar_wait(&sm.full[w][get], parity, &g_kv8_error)) {
+    const int32_t stop = int32_t(min(int64_t(c.n), c.at + (end - c.unit)));
+    for (; c.at < stop; ++c.at, ++c.unit) {
+      if (!__all_sync(FULL_MASK, mbar_wait(&sm.full[w][get], parity, &g_kv8_error))) {
         // leave nothing in flight: the other copies of this warp, each again bounded
         for (int s = 0; s < AS; ++s) {
           const int x = get + s < AS ? get + s : get + s - AS;
@@ -633,64 +649,78 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
         return;
       }
       const int valid = sm.valid[w][get];
-      const uint8_t* block = sm.stage[w][get];
-      if (valid > 0) {
-        const float2 sc = *reinterpret_cast<const float2*>(block);
-        const uint4* kc = reinterpret_cast<const uint4*>(block + HEAD_BYTES) + lane;
-        const uint4* vc = kc + D;
-        float acc[2][4] = {};
+      const uint8_t* step = sm.stage[w][get];
+      // x[b][0], [1]: block b's token rho, columns 2t, 2t + 1; [2], [3]: token rho + 2
+      const int rho = 4 * (g >> 1) + (g & 1);
+      float x[GB][4], lsv[GB], top[2] = {-INFINITY, -INFINITY}, top_v[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < KS / 2; ++i) {
-          const uint4 x = kc[32 * i];
-          mma_f16(acc[0], codes_lo(x.x), codes_lo(x.y), codes_hi(x.x), codes_hi(x.y), qf[2 * i][0],
-                  qf[2 * i][1]);
-          mma_f16(acc[1], codes_lo(x.z), codes_lo(x.w), codes_hi(x.z), codes_hi(x.w),
-                  qf[2 * i + 1][0], qf[2 * i + 1][1]);
+      for (int b = 0; b < GB; ++b) {
+        x[b][0] = x[b][1] = x[b][2] = x[b][3] = -INFINITY;
+        lsv[b] = 0.0f;
+        if (b * BT < valid) {
+          const uint8_t* block = step + b * block_bytes(D);
+          const float2 sc = *reinterpret_cast<const float2*>(block);
+          const uint4* kc = reinterpret_cast<const uint4*>(block + HEAD_BYTES) + lane;
+          float acc[2][4] = {};
+#pragma unroll
+          for (int i = 0; i < KS / 2; ++i) {
+            const uint4 y = kc[32 * i];
+            mma_f16(acc[0], codes_lo(y.x), codes_lo(y.y), codes_hi(y.x), codes_hi(y.y), qf[2 * i][0],
+                    qf[2 * i][1]);
+            mma_f16(acc[1], codes_lo(y.z), codes_lo(y.w), codes_hi(y.z), codes_hi(y.w),
+                    qf[2 * i + 1][0], qf[2 * i + 1][1]);
+          }
+          lsv[b] = float(int((__float_as_uint(sc.y) >> 23) & 0xffu) - 127);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            x[b][j] = (acc[0][j] + acc[1][j]) * qs[j & 1] * sc.x;
+            if (b * BT + rho + (j & 2) >= valid) x[b][j] = -INFINITY;
+            top[j & 1] = fmaxf(top[j & 1], x[b][j]);
+            top_v[j & 1] = fmaxf(top_v[j & 1], x[b][j] + lsv[b]);
+          }
         }
-        // acc[.][0], [1]: token rho, columns 2t, 2t + 1; [2], [3]: token rho + 2
-        const int rho = 4 * (g >> 1) + (g & 1);
-        const float lsv = float(int((__float_as_uint(sc.y) >> 23) & 0xffu) - 127);
-        float x[4];
-        bool move = false;
+      }
+      const bool move = top[0] > m[0] + LAZY_M || top[1] > m[1] + LAZY_M ||
+                        top_v[0] > r[0] + LAZY_R || top_v[1] > r[1] + LAZY_R;
+      if (__any_sync(FULL_MASK, move)) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          x[j] = (acc[0][j] + acc[1][j]) * qs[j & 1] * sc.x;
-          if (rho + (j & 2) >= valid) x[j] = -INFINITY;
-          move |= x[j] > m[j & 1] + LAZY_M || x[j] + lsv > r[j & 1] + LAZY_R;
-        }
-        if (__any_sync(FULL_MASK, move)) {
+        for (int j = 0; j < 2; ++j) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            float top = fmaxf(x[j], x[j + 2]);
-            top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, 4));
-            top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, 8));
-            top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, 16));
-            const float m1 = fmaxf(m[j], top), r1 = fmaxf(r[j], top + lsv - TOP_R);
-            if (m1 > m[j]) {
-              l[j] *= ex2(m[j] - m1);
-              m[j] = m1;
-            }
-            if (r1 > r[j]) {
-              const float f = ex2(r[j] - r1);
-              r[j] = r1;
+          for (int d = 4; d < 32; d <<= 1) {
+            top[j] = fmaxf(top[j], __shfl_xor_sync(FULL_MASK, top[j], d));
+            top_v[j] = fmaxf(top_v[j], __shfl_xor_sync(FULL_MASK, top_v[j], d));
+          }
+          const float m1 = fmaxf(m[j], top[j]), r1 = fmaxf(r[j], top_v[j] - TOP_R);
+          if (m1 > m[j]) {
+            l[j] *= ex2(m[j] - m1);
+            m[j] = m1;
+          }
+          if (r1 > r[j]) {
+            const float f = ex2(r[j] - r1);
+            r[j] = r1;
 #pragma unroll
-              for (int s = 0; s < KS; ++s) {
-                o[s][j] *= f;
-                o[s][j + 2] *= f;
-              }
+            for (int s = 0; s < KS; ++s) {
+              o[s][j] *= f;
+              o[s][j + 2] *= f;
             }
           }
         }
+      }
+#pragma unroll
+      for (int b = 0; b < GB; ++b) {
+        if (b * BT >= valid) break;
         float y[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const bool in = rho + (j & 2) < valid;
-          l[j & 1] += in ? ex2(x[j] - m[j & 1]) : 0.0f;
-          y[j] = in ? ex2(x[j] + lsv - r[j & 1]) : 0.0f;
+          const bool in = b * BT + rho + (j & 2) < valid;
+          l[j & 1] += in ? ex2(x[b][j] - m[j & 1]) : 0.0f;
+          y[j] = in ? ex2(x[b][j] + lsv[b] - r[j & 1]) : 0.0f;
           if (PAIRED && t >= 2) y[j] -= __half2float(__float2half_rn(y[j]));
         }
         const uint32_t b0 = transpose8(pack_f16(y[0], y[1]));
         const uint32_t b1 = transpose8(pack_f16(y[2], y[3]));
+        const uint4* vc =
+            reinterpret_cast<const uint4*>(step + b * block_bytes(D) + HEAD_BYTES) + D + lane;
 #pragma unroll
         for (int i = 0; i < KS / 2; ++i) {
           const uint4 v = vc[32 * i];
@@ -706,8 +736,8 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
 
     // ---- the pair's result, or its record
     const int32_t seq = c.seq, kvh = c.head;
-    const int64_t pair_end = c.unit - c.blk + c.nb;  // its last block's unit, plus one
-    const bool done = c.blk == c.nb, whole = done && blk0 == 0;
+    const int64_t pair_end = c.unit - c.at + c.n;  // its last step's unit, plus one
+    const bool done = c.at == c.n, whole = done && from == 0;
     if (done && c.unit < end) {
       c.next_pair(a);
       load_q();
@@ -755,7 +785,7 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
       }
     }
     // the range that a pair starts in says what there is to merge
-    if (lane == 0 && blk0 == 0 && (!done || a.by_pair)) {
+    if (lane == 0 && from == 0 && (!done || a.by_pair)) {
       const int64_t last = quotient(pair_end - 1, per);
       a.owner[a.by_pair ? seq * a.kv_heads + kvh : wid] =
           make_int4(seq, kvh, done ? 0 : int(last) - wid + 1, 2 * wid + (first ? 0 : 1));
@@ -772,6 +802,7 @@ __global__ void __launch_bounds__(32 * AW) kv8_attn_kernel(const Kv8AttnArgs a) 
 template <int D, int CHUNK>
 __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnArgs a) {
   constexpr int LANES = CHUNK / 4, SLOTS = 256 / LANES;
+  constexpr int AHEAD = CHUNK == 32 ? 8 : 2;  // of a thread's records, loaded with the heads
   __shared__ float4 part[SLOTS][LANES];
   __shared__ float fac[MAX_WARPS];
   __shared__ float2 top_s[8];
@@ -794,7 +825,6 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnArgs a) {
   const auto values = [&](int i) {
     return *reinterpret_cast<const float4*>(rec(i) + 4 + CHUNK * blockIdx.z + 4 * quad);
   };
-  constexpr int AHEAD = 4;  // of this thread's records, loaded with the heads
   float4 ahead[AHEAD];
 #pragma unroll
   for (int j = 0; j < AHEAD; ++j)
@@ -866,7 +896,7 @@ cudaError_t launch_attn(Kv8AttnArgs a, cudaStream_t s) {
       e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kv8_attn_kernel<D, PAIRED>, 32 * AW,
                                                         sizeof(AttnSmem<D>));
     if (e != cudaSuccess) return e;
-    grid = std::max(1, std::min(sms * per, MAX_WARPS / AW));
+    grid = std::max(1, std::min(sms * std::min(per, ctas_per_sm(D)), MAX_WARPS / AW));
     if (dev < 64) ctas[dev].store(grid, std::memory_order_relaxed);
     configured.mark(dev);
   }
@@ -876,9 +906,9 @@ cudaError_t launch_attn(Kv8AttnArgs a, cudaStream_t s) {
   const int entries = a.by_pair ? int(pairs) : warps;
   e = launch_dependent(kv8_attn_kernel<D, PAIRED>, dim3(grid), 32 * AW, sizeof(AttnSmem<D>), s, a);
   if (e != cudaSuccess) return e;
-  // few heads have many records each: then 64 dims to a CTA, 16 threads along them
+  // few heads have many records each: then 32 dims to a CTA, 32 threads along them
   if (entries * a.group <= 256)
-    return launch_dependent(kv8_merge_kernel<D, 64>, dim3(entries, a.group, D / 64), 256, 0, s, a);
+    return launch_dependent(kv8_merge_kernel<D, 32>, dim3(entries, a.group, D / 32), 256, 0, s, a);
   return launch_dependent(kv8_merge_kernel<D, D>, dim3(entries, a.group, 1), 256, 0, s, a);
 }
 

@@ -409,6 +409,23 @@ def test_attention_batches_and_long_contexts(qcache, n, length, kv, group, dim):
     qcache.kv8_check()
 
 
+@pytest.mark.parametrize("lens,kv,group,dim", [
+    ([16000] * 5, 4, 4, 256), ([90000], 4, 4, 256), ([20000] * 16, 2, 8, 128), ([700] * 9 + [0, 1] + [30011] * 12, 2, 2, 128),
+    ([5] * 60 + [65536] * 4, 4, 1, 64), ([40] * 200 + [9000] * 30, 8, 4, 64)])
+def test_attention_large_batches_repeat_their_bits(qcache, lens, kv, group, dim):
+    """Enough blocks for the small ranges that CTAs draw as they get ready: the
+    results are right, and the same bits whoever drew what."""
+    pool, kvs, g = filled(qcache, lens, kv, dim, seed=len(lens))
+    q = rows_of(g, len(lens), kv * group, dim)
+    got = attend(qcache, pool.cache, pool.table, lens, q)
+    qcache.kv8_check()
+    check_attention(got, q, None, kvs, dim ** -0.5)
+    for _ in range(5):
+        again = attend(qcache, pool.cache, pool.table, lens, q)
+        assert torch.equal(got.view(torch.int16), again.view(torch.int16))
+    qcache.kv8_check()
+
+
 def test_attention_one_long_among_short(qcache):
     lens = [3, 20000, 0, 1, 640, 64, 0, 2]
     pool, kvs, g = filled(qcache, lens, 4, 256, seed=9)
