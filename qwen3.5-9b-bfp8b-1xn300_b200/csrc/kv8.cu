@@ -156,7 +156,46 @@ __global__ void __launch_bounds__(32 * TW, WRITE ? 4 : 1) kv8_rows_kernel(const 
   int seq;
   int64_t nth = 0;  // of the sequence's touched blocks
   int64_t first = 0, row0 = 0, cnt = 1;  // its first position, row and number of rows
-  if (a.start) {
+  if (a.start && a.n <= 128) {
+    // every warp looks for itself, 32 sequences at a time, without a barrier
+    const uint32_t most = gridDim.x * PAIRS;  // blocks of a sequence beyond that are out of any CTA's reach
+    uint32_t before = 0;
+    seq = -1;
+    for (int i0 = 0; i0 < a.n; i0 += 32) {
+      const int i = min(i0 + lane, a.n - 1);
+      const int32_t p = a.pos[i], r = a.start[i];
+      const int64_t c = i0 + lane < a.n ? int64_t(a.start[i + 1]) - r : 0;
+      if (c > 0 && p < 0) record_error(&g_kv8_error, QC_ERR_BOUNDS);
+      const uint32_t nb = p < 0 ? 0 : uint32_t(min(blocks_touched(p, c), int64_t(most)));
+      uint32_t upto = nb;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const uint32_t x = __shfl_up_sync(FULL_MASK, upto, m);
+        if (lane >= m) upto += x;
+      }
+      upto = min(upto, most);  // at most 32 * 2^26 before, however the rows overlap
+#pragma unroll
+      for (int x = 0; x < TILES; ++x) {
+        const uint32_t b = __shfl_sync(FULL_MASK, ub, x * LPT);
+        const int in = __popc(__ballot_sync(FULL_MASK, before + upto <= b));  // sequences that end before b
+        const int from = min(in, 31);
+        const int64_t c1 = __shfl_sync(FULL_MASK, c, from);
+        const int32_t p1 = __shfl_sync(FULL_MASK, p, from), r1 = __shfl_sync(FULL_MASK, r, from);
+        const uint32_t past = __shfl_sync(FULL_MASK, upto - nb, from);
+        if (tile == x && seq < 0 && in < 32 && b >= before) {
+          seq = i0 + in;
+          nth = b - before - past;
+          first = p1;
+          row0 = r1;
+          cnt = c1;
+        }
+      }
+      before += __shfl_sync(FULL_MASK, upto, 31);
+    }
+    if (seq >= a.n) seq = -1;
+    if (blockIdx.x == 0 && tid == 0 && uint64_t(before) * heads > uint64_t(gridDim.x) * PAIRS)
+      record_error(&g_kv8_error, QC_ERR_BOUNDS);
+  } else if (a.start) {
     const auto count = [&](int i) -> int64_t {
       const int64_t cnt = int64_t(a.start[i + 1]) - a.start[i];
       if (cnt > 0 && a.pos[i] < 0) record_error(&g_kv8_error, QC_ERR_BOUNDS);
@@ -974,7 +1013,8 @@ int rows_call(const char* call, bool write, const qc_kv8_cache* c, const int32_t
       start ? std::min<int64_t>(rows, int64_t(rows) / BT + 2 * int64_t(n)) : int64_t(n);
   const int64_t per_cta = TW / 2 * (256 / c->head_dim);
   const int64_t ctas = (blocks * c->n_kv_heads + per_cta - 1) / per_cta;
-  if (ctas * per_cta > INT32_MAX) return refuse(QC_ERR_ARG, "%s: %d rows of %d heads", call, rows, c->n_kv_heads);
+  if (ctas * per_cta > 1 << 26)  // over 256 GB of rows
+    return refuse(QC_ERR_ARG, "%s: %d rows of %d heads", call, rows, c->n_kv_heads);
   const dim3 grid((unsigned)ctas);
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e;
