@@ -468,7 +468,7 @@ struct AttnSmem {
   alignas(8) uint64_t full[AW][AS];
   int32_t valid[AW][AS];                                 // tokens of the step; 0: nothing was copied
   int64_t sums[AW];
-  struct { int64_t unit; int32_t seq, n, len; } start[AW];  // the sequence a warp starts in, its first unit
+  struct { int64_t unit; int32_t seq, n, len; } start[AW];
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -561,33 +561,59 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
   extern __shared__ __align__(128) uint8_t smem_raw[];
   AttnSmem<D>& sm = *reinterpret_cast<AttnSmem<D>*>(smem_raw);
   constexpr int KS = D / 16;  // steps of 16 dims
-  constexpr int AS = stages(D), GB = step_blocks(D);
+  constexpr int AS = stages(D), GB = step_blocks(D), ST = BT * GB;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
   if (lane == 0) {
     for (int s = 0; s < AS; ++s) mbar_init(&sm.full[w][s], 1);
     fence_mbar_init();
   }
+  __syncwarp();  // a warp's barriers are its own
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   const int warps = gridDim.x * AW, wid = w * gridDim.x + blockIdx.x;
-  const auto count = [&](int i) { return seq_steps<D>(a, i); };
-  int64_t before, mine, total;
-  scan_blocks<AW>(a.n, count, sm.sums, before, mine, total);
-  total *= a.kv_heads;
-  const int64_t per = max(quotient(total + warps - 1, warps), int64_t(1));
-  for (int x = 0; x < AW; ++x) {
-    const int64_t u = (int64_t(x) * gridDim.x + blockIdx.x) * per;  // warp x's first step
-    if (u >= before * a.kv_heads && u < (before + mine) * a.kv_heads) {
-      int64_t at = before;
-      int i = tid * ((a.n + 32 * AW - 1) / (32 * AW));
-      int64_t nb = count(i);
-      for (; u >= (at + nb) * a.kv_heads; nb = count(++i)) at += nb;
-      sm.start[x] = {at * a.kv_heads, i, int32_t(nb), seq_len(a, i)};
+  int64_t total, per;
+  const auto share = [&]() { per = max(quotient(total + warps - 1, warps), int64_t(1)); };
+  struct { int64_t unit; int32_t seq, n, len; } start;  // the sequence this warp starts in, its first unit
+  if (a.n <= 32) {  // a sequence per lane, every warp for itself
+    const int32_t len = seq_len(a, min(lane, a.n - 1));
+    const int32_t steps = lane < a.n ? int32_t((int64_t(len) + ST - 1) / ST) : 0;
+    int64_t upto = steps;
+#pragma unroll
+    for (int m = 1; m < 32; m <<= 1) {
+      const int64_t x = __shfl_up_sync(FULL_MASK, upto, m);
+      if (lane >= m) upto += x;
     }
+    total = __shfl_sync(FULL_MASK, upto, 31) * a.kv_heads;
+    share();
+    const int in = min(__popc(__ballot_sync(FULL_MASK, upto * a.kv_heads <= wid * per)), 31);
+    start.unit = __shfl_sync(FULL_MASK, upto - steps, in) * a.kv_heads;
+    start.seq = in;
+    start.n = __shfl_sync(FULL_MASK, steps, in);
+    start.len = __shfl_sync(FULL_MASK, len, in);
+  } else {
+    const auto count = [&](int i) { return seq_steps<D>(a, i); };
+    int64_t before, mine;
+    scan_blocks<AW>(a.n, count, sm.sums, before, mine, total);
+    total *= a.kv_heads;
+    share();
+    for (int x = 0; x < AW; ++x) {
+      const int64_t u = (int64_t(x) * gridDim.x + blockIdx.x) * per;  // warp x's first step
+      if (u >= before * a.kv_heads && u < (before + mine) * a.kv_heads) {
+        int64_t at = before;
+        int i = tid * ((a.n + 32 * AW - 1) / (32 * AW));
+        int64_t nb = count(i);
+        for (; u >= (at + nb) * a.kv_heads; nb = count(++i)) at += nb;
+        sm.start[x] = {at * a.kv_heads, i, int32_t(nb), seq_len(a, i)};
+      }
+    }
+    __syncthreads();
+    start.unit = sm.start[w].unit;
+    start.seq = sm.start[w].seq;
+    start.n = sm.start[w].n;
+    start.len = sm.start[w].len;
   }
-  __syncthreads();
   const int64_t begin = wid * per, end = min(begin + per, total);
   if (lane == 0 && !a.by_pair) a.owner[wid] = make_int4(0, 0, 0, 0);
   if (begin >= end) {
@@ -597,11 +623,11 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
 
   Cursor<D> c;
   c.unit = begin;
-  c.seq = sm.start[w].seq;
-  c.n = sm.start[w].n;
-  c.len = sm.start[w].len;
-  c.head = int32_t(quotient(begin - sm.start[w].unit, c.n));
-  c.at = int32_t(begin - sm.start[w].unit - int64_t(c.head) * c.n);
+  c.seq = start.seq;
+  c.n = start.n;
+  c.len = start.len;
+  c.head = int32_t(quotient(begin - start.unit, c.n));
+  c.at = int32_t(begin - start.unit - int64_t(c.head) * c.n);
   Cursor<D> p = c;  // the copies run AS steps ahead
   int put = 0;
   auto issue = [&]() {  // lane 0: the copy of step p into the next stage

@@ -515,13 +515,17 @@ class Rope:
         cfg = RopeConfig(rot_dim, layout, scaling, orig_ctx, base, factor, beta_fast, beta_slow,
                          mscale)
         self.freq = RopeFrequencies()
-        _ck_thread(lib().qc_rope_init(C.byref(cfg), C.byref(self.freq)))
+        self._L = lib()
+        self._freq = C.byref(self.freq)
+        _ck_thread(self._L.qc_rope_init(C.byref(cfg), self._freq))
 
     def apply(self, head_dim, pos_ptr, n_rows, parts, eps=1e-6, stream=0):
         """qc_rope_apply over a list of RopePart."""
-        arr = (RopePart * len(parts))(*parts)
-        _ck_thread(lib().qc_rope_apply(C.byref(self.freq), head_dim, eps, pos_ptr, n_rows, arr,
-                                       len(parts), stream))
+        n = len(parts)
+        rc = self._L.qc_rope_apply(self._freq, head_dim, eps, pos_ptr, n_rows,
+                                   (RopePart * n)(*parts), n, stream)
+        if rc:
+            _ck_thread(rc)
 
 
 def kv8_page_bytes(n_kv_heads, head_dim) -> int:
@@ -539,24 +543,33 @@ class Kv8Cache:
 
     def __init__(self, pool_ptr, n_pages, n_kv_heads, head_dim):
         self.desc = Kv8Desc(pool_ptr, n_pages, n_kv_heads, head_dim, 0)
+        self._L = lib()
+        self._desc = C.byref(self.desc)
 
     def write(self, table_ptr, pt_stride, pos_ptr, row_start_ptr, n, n_rows, k_ptr, k_ld, v_ptr,
               v_ld, stream=0):
         """qc_kv8_write; row_start_ptr 0: one row per sequence."""
-        _ck_thread(lib().qc_kv8_write(C.byref(self.desc), table_ptr, pt_stride, pos_ptr,
-                                      row_start_ptr, n, n_rows, k_ptr, k_ld, v_ptr, v_ld, stream))
+        rc = self._L.qc_kv8_write(self._desc, table_ptr, pt_stride, pos_ptr, row_start_ptr, n,
+                                  n_rows, k_ptr, k_ld, v_ptr, v_ld, stream)
+        if rc:
+            _ck_thread(rc)
 
     def read(self, table_ptr, pt_stride, pos_ptr, row_start_ptr, n, n_rows, k_ptr, k_ld, v_ptr,
              v_ld, stream=0):
-        _ck_thread(lib().qc_kv8_read(C.byref(self.desc), table_ptr, pt_stride, pos_ptr,
-                                     row_start_ptr, n, n_rows, k_ptr, k_ld, v_ptr, v_ld, stream))
+        """qc_kv8_read; arguments as write."""
+        rc = self._L.qc_kv8_read(self._desc, table_ptr, pt_stride, pos_ptr, row_start_ptr, n,
+                                 n_rows, k_ptr, k_ld, v_ptr, v_ld, stream)
+        if rc:
+            _ck_thread(rc)
 
     def attn_workspace_bytes(self, n, n_head) -> int:
-        return lib().qc_kv8_attn_workspace_bytes(C.byref(self.desc), n, n_head)
+        return self._L.qc_kv8_attn_workspace_bytes(self._desc, n, n_head)
 
     def attn_decode(self, table_ptr, pt_stride, len_ptr, n, n_head, q_ptr, q_ld, q_head, gate_ptr,
                     scale, out_ptr, out_ld, workspace_ptr, workspace_bytes, stream=0):
         """qc_kv8_attn_decode; gate_ptr 0: no output gate."""
-        _ck_thread(lib().qc_kv8_attn_decode(C.byref(self.desc), table_ptr, pt_stride, len_ptr, n,
-                                            n_head, q_ptr, q_ld, q_head, gate_ptr, scale, out_ptr,
-                                            out_ld, workspace_ptr, workspace_bytes, stream))
+        rc = self._L.qc_kv8_attn_decode(self._desc, table_ptr, pt_stride, len_ptr, n, n_head,
+                                        q_ptr, q_ld, q_head, gate_ptr, scale, out_ptr, out_ld,
+                                        workspace_ptr, workspace_bytes, stream)
+        if rc:
+            _ck_thread(rc)
