@@ -97,6 +97,7 @@ int qc_kv8_read(const qc_kv8_cache* cache, const int32_t* page_table_dev, int32_
  *   out_dev    bf16 [n_head][head_dim] per sequence at i * out_ld; 16-byte
  *              aligned, out_ld a multiple of 8
  * n_head is a multiple of n_kv_heads, at most QC_KV8_MAX_GROUP times it.
+ * out must not overlap q, the gate or the pool.
  * workspace: at least qc_kv8_attn_workspace_bytes bytes of device memory, 16-
  * byte aligned, for this call alone while it runs; its contents do not matter.
  * Products are exact to f32 and sums are kept in f32; a NaN or infinity in q

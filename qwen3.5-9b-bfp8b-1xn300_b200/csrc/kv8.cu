@@ -445,7 +445,7 @@ struct Kv8AttnArgs {
   int64_t q_ld, q_head, out_ld;
   float scale;      // scale * log2(e)
   int32_t n_pages, pt_stride, kv_heads, group, n;
-  int32_t by_pair;
+  int32_t by_pair, warps;
 };
 
 constexpr int AW = 4;                                    // warps per CTA
@@ -876,8 +876,13 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int4 own = a.owner[blockIdx.x];
-  const int n = min(own.z, MAX_WARPS);
+  const int n = own.z;
   if (n == 0) return;
+  // an entry whose warp gave up on a wait is whatever the workspace held: follow it
+  // only inside the records and the batch
+  if (n < 0 || n > a.warps || own.w < 0 || own.w / 2 > a.warps - n || own.x < 0 || own.x >= a.n ||
+      own.y < 0 || own.y >= a.kv_heads)
+    return;
   const int64_t step = int64_t(a.group) * (D + 4);
   auto rec = [&](int i) {
     return a.rec + (i == 0 ? own.w : 2 * (own.w / 2 + i)) * step + h * (D + 4);
@@ -968,6 +973,7 @@ cudaError_t launch_attn(Kv8AttnArgs a, cudaStream_t s) {
   const int warps = grid * AW;
   const int64_t pairs = int64_t(a.n) * a.kv_heads;
   a.by_pair = pairs <= warps;
+  a.warps = warps;
   const int entries = a.by_pair ? int(pairs) : warps;
   e = launch_dependent(kv8_attn_kernel<D, PAIRED>, dim3(grid), 32 * AW, sizeof(AttnSmem<D>), s, a);
   if (e != cudaSuccess) return e;

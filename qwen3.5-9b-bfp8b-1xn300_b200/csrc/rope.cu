@@ -341,7 +341,7 @@ extern "C" int qc_rope_apply(const qc_rope* rope, int32_t head_dim, float eps,
     a.chunk = (most + 3) / 4 * 4;
     while (a.chunk > 4 && int64_t(n_rows) * a.gl * slices(a.chunk) < WANT)
       a.chunk = (a.chunk / 2 + 3) / 4 * 4;
-    const bool few = int64_t(n_rows) * a.gl * slices(a.chunk) < FEW;
+    const bool few = int64_t(n_rows) * a.gl * slices(a.chunk) < FEW && slices(1) < 65536;
     if (few) a.chunk = 1;
     const dim3 grid((unsigned)((int64_t(n_rows) * a.gl + qc::RT - 1) / qc::RT),
                     (unsigned)slices(a.chunk));

@@ -591,3 +591,39 @@ def test_captured_steps_and_two_graphs_at_once(qcache):
             k, v = s["pool"].read([0] * n, now)
             check_attention(s["out"], s["q"], None, list(zip(k.split(now), v.split(now))), dim ** -0.5)
     qcache.kv8_check()
+
+
+def test_first_calls_of_a_process_may_be_captured(qcache):
+    """Kernel attributes, occupancy and module loading on the first call of a
+    process, all inside a capture."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import importlib.util, torch
+spec = importlib.util.spec_from_file_location("qcache", PATH)
+qc = importlib.util.module_from_spec(spec)
+spec.loader.exec_module(qc)
+pool = torch.zeros(4 * qc.kv8_page_bytes(2, 128), dtype=torch.uint8, device="cuda")
+c = qc.Kv8Cache(pool.data_ptr(), 4, 2, 128)
+table, pos, ln = torch.zeros(3, 1, dtype=torch.int32, device="cuda").unbind(0)
+ln = ln + 1
+k, q = torch.ones(1, 2, 128, device="cuda").bfloat16(), torch.ones(1, 8, 128, device="cuda").bfloat16()
+out = torch.zeros_like(q)
+ws = torch.empty(c.attn_workspace_bytes(1, 8), dtype=torch.uint8, device="cuda")
+rope, g = qc.Rope(64), torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(g):
+    st = torch.cuda.current_stream().cuda_stream
+    rope.apply(128, pos.data_ptr(), 1, [qc.RopePart(k.data_ptr(), k.data_ptr(), 2, 256, 128, 256, 128)], 1e-6, st)
+    c.write(table.data_ptr(), 1, pos.data_ptr(), 0, 1, 1, k.data_ptr(), 256, k.data_ptr(), 256, st)
+    c.attn_decode(table.data_ptr(), 1, ln.data_ptr(), 1, 8, q.data_ptr(), 1024, 128, 0, 0.1, out.data_ptr(), 1024,
+                  ws.data_ptr(), ws.numel(), st)
+g.replay()
+qc.kv8_check(st)
+assert bool((out == 1).all())
+"""
+    code = code.replace("PATH", repr(os.path.abspath(qcache.__file__)))
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr[-2000:]

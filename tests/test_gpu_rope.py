@@ -60,6 +60,7 @@ def parts_of(qcache, q, k, qo, ko, qw, kw):
 @pytest.mark.parametrize("dim,rot,nq,nk,rows", [
     (256, 64, 16, 4, 9), (256, 256, 3, 1, 33), (128, 128, 32, 8, 5), (64, 64, 5, 5, 200), (64, 16, 7, 1, 1),
     (128, 24, 9, 3, 17), (96, 96, 6, 2, 11), (8, 2, 1, 1, 3), (40, 38, 2, 70, 4), (256, 254, 1, 1, 65), (256, 64, 16, 4, 3001),
+    (64, 64, 16, 16, 20000), (8, 8, 16384, 16384, 1),
 ])
 def test_matches_64_bits(qcache, dim, rot, nq, nk, rows, norm, half):
     g = torch.Generator(device="cuda")
@@ -101,6 +102,28 @@ def test_projection_rows_in_place_and_untouched_neighbours(qcache):
     check(k, *reference(before[:, 8192:9216].unflatten(1, (4, 256)), pos, f, 1.0, 64, True, kw))
     assert torch.equal(proj[:, :8192].unflatten(1, (16, 512))[:, :, 256:].view(torch.int16), b[:, :, 256:].view(torch.int16))
     assert torch.equal(proj[:, 9216:].view(torch.int16), before[:, 9216:].view(torch.int16))
+
+
+def test_four_parts_with_and_without_norm(qcache):
+    """Parts of different sizes in one launch; one reads a single row's heads
+    out of order (a negative head stride)."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(8)
+    rows, dim, heads = 70, 128, [3, 1, 17, 6]
+    pos = positions(rows, 2)
+    rope = qcache.Rope(128, layout=qcache.ROPE_INTERLEAVED, base=1e4, scaling=qcache.ROPE_NTK, factor=8.0)
+    f = list(rope.freq.inv_freq[:64])
+    xs = [torch.randn(rows, h, dim, generator=g, device="cuda").bfloat16() for h in heads]
+    outs = [torch.empty_like(x) for x in xs]
+    ws = [1 + 0.1 * torch.randn(dim, generator=g, device="cuda"), None, None, torch.ones(dim, device="cuda")]
+    parts = [qcache.RopePart(x.data_ptr(), o.data_ptr(), h, x.stride(0), dim, o.stride(0), dim, w.data_ptr() if w is not None else 0)
+             for x, o, h, w in zip(xs, outs, heads, ws)]
+    parts[3].x, parts[3].x_head = xs[3].data_ptr() + 2 * 5 * dim, -dim
+    rope.apply(dim, pos.data_ptr(), rows, parts, EPS)
+    torch.cuda.synchronize()
+    xs[3] = xs[3].flip(1)
+    for x, o, w in zip(xs, outs, ws):
+        check(o, *reference(x, pos, f, 1.0, 128, False, w))
 
 
 def test_position_zero_without_norm_keeps_the_bits(qcache):
