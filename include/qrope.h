@@ -85,10 +85,9 @@ int qc_rope_init(const qc_rope_config* cfg, qc_rope* rope);
 typedef struct qc_rope_part {
   const uint16_t* x;     /* bf16, device */
   uint16_t* out;         /* bf16, device */
-  const float* norm_w;   /* [head_dim] f32, device; NULL: no norm */
+  int64_t n_heads;       /* 1 .. QC_ROPE_MAX_HEADS */
   int64_t x_ld, x_head, out_ld, out_head;
-  int32_t n_heads;       /* 1 .. QC_ROPE_MAX_HEADS */
-  int32_t reserved;      /* 0 */
+  const float* norm_w;   /* [head_dim] f32, device; NULL: no norm */
 } qc_rope_part;
 
 /* Applies the rotation to n_parts groups of n_rows rows in one launch.

@@ -26,26 +26,41 @@ inline int refuse(int code, const char* fmt, ...) {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// A kernel launched here may follow `p`: it is device memory of the current
-// device (a host pointer, or one of another device, would fault the kernel).
-inline int check_device_pointer(const char* call, const char* name, const void* p) {
-  if (!p) return refuse(QC_ERR_ARG, "%s: %s is null", call, name);
-  int dev = 0;
-  cudaPointerAttributes at{};
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaPointerGetAttributes(&at, p);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    return refuse(QC_ERR_CUDA, "%s: %s: %s", call, name, cudaGetErrorString(e));
+// The buffers of a call, each of which a kernel launched here may follow: device
+// memory of the current device (a host pointer, or one of another device, would
+// fault the kernel).  The first one that is not decides what check() returns.
+class BufferCheck {
+ public:
+  explicit BufferCheck(const char* call) : call_(call) {}
+  BufferCheck& need(const char* name, const void* p) {
+    if (rc_) return *this;
+    if (!p) return fail(QC_ERR_ARG, name, "is null");
+    return maybe(name, p);
   }
-  if (at.type == cudaMemoryTypeManaged) return QC_OK;
-  if (at.type != cudaMemoryTypeDevice)
-    return refuse(QC_ERR_ARG, "%s: %s is not device memory", call, name);
-  if (at.device != dev)
-    return refuse(QC_ERR_ARG, "%s: %s is on device %d, the current one is %d", call, name,
-                  at.device, dev);
-  return QC_OK;
-}
+  BufferCheck& maybe(const char* name, const void* p) {  // null is fine
+    if (rc_ || !p) return *this;
+    cudaPointerAttributes at{};
+    cudaError_t e = dev_ < 0 ? cudaGetDevice(&dev_) : cudaSuccess;
+    if (e == cudaSuccess) e = cudaPointerGetAttributes(&at, p);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      return fail(QC_ERR_CUDA, name, cudaGetErrorString(e));
+    }
+    if (at.type == cudaMemoryTypeManaged) return *this;
+    if (at.type != cudaMemoryTypeDevice) return fail(QC_ERR_ARG, name, "is not device memory");
+    if (at.device != dev_) return fail(QC_ERR_ARG, name, "is not on the current device");
+    return *this;
+  }
+  int check() const { return rc_; }
+
+ private:
+  BufferCheck& fail(int code, const char* name, const char* why) {
+    rc_ = refuse(code, "%s: %s %s", call_, name, why);
+    return *this;
+  }
+  const char* call_;
+  int dev_ = -1, rc_ = QC_OK;
+};
 
 // Launch as a programmatic dependent of the kernel before: it may start early and
 // waits (griddepcontrol.wait) before it reads or writes memory.

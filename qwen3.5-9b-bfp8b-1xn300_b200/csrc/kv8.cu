@@ -993,14 +993,11 @@ int check_cache(const char* call, const qc_kv8_cache* c) {
   return QC_OK;
 }
 
-int check_table(const char* call, const qc_kv8_cache* c, const int32_t* table, int32_t pt_stride,
-                int32_t n) {
+int check_table(const char* call, int32_t pt_stride, int32_t n) {
   if (n < 0 || n > QC_KV8_MAX_SEQS)
     return refuse(QC_ERR_ARG, "%s: %d sequences, limit is %d", call, n, QC_KV8_MAX_SEQS);
   if (pt_stride < 1) return refuse(QC_ERR_ARG, "%s: pt_stride %d", call, pt_stride);
-  if (n == 0) return QC_OK;
-  const int rc = check_device_pointer(call, "the pool", c->pool);
-  return rc ? rc : check_device_pointer(call, "page_table_dev", table);
+  return QC_OK;
 }
 
 int rows_call(const char* call, bool write, const qc_kv8_cache* c, const int32_t* table,
@@ -1017,13 +1014,17 @@ int rows_call(const char* call, bool write, const qc_kv8_cache* c, const int32_t
                   (long long)k_ld, (long long)v_ld, (long long)width);
   if (!aligned16(k) || !aligned16(v))
     return refuse(QC_ERR_ARG, "%s: k and v must be 16-byte aligned", call);
-  rc = check_table(call, c, table, pt_stride, n);
+  rc = check_table(call, pt_stride, n);
+  if (rc || n == 0 || rows == 0) return rc;
+  rc = BufferCheck(call)
+           .need("the pool", c->pool)
+           .need("page_table_dev", table)
+           .need("pos_dev", pos)
+           .maybe("row_start_dev", start)
+           .need("k_dev", k)
+           .need("v_dev", v)
+           .check();
   if (rc) return rc;
-  if (n == 0 || rows == 0) return QC_OK;
-  if ((rc = check_device_pointer(call, "pos_dev", pos))) return rc;
-  if (start && (rc = check_device_pointer(call, "row_start_dev", start))) return rc;
-  if ((rc = check_device_pointer(call, "k_dev", k))) return rc;
-  if ((rc = check_device_pointer(call, "v_dev", v))) return rc;
 
   Kv8RowsArgs a{};
   a.pool = c->pool;
@@ -1122,17 +1123,22 @@ extern "C" int qc_kv8_attn_decode(const qc_kv8_cache* cache, const int32_t* page
   if (!qc::aligned16(q_dev) || !qc::aligned16(gate_dev) || !qc::aligned16(out_dev) ||
       !qc::aligned16(workspace))
     return qc::refuse(QC_ERR_ARG, "%s: q, gate, out and workspace must be 16-byte aligned", CALL);
-  rc = qc::check_table(CALL, cache, page_table_dev, pt_stride, n);
+  rc = qc::check_table(CALL, pt_stride, n);
   if (rc || n == 0) return rc;
   const int64_t need = qc_kv8_attn_workspace_bytes(cache, n, n_head);
   if (workspace_bytes < need)
     return qc::refuse(QC_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", CALL,
                       (long long)workspace_bytes, (long long)need);
-  if ((rc = qc::check_device_pointer(CALL, "len_dev", len_dev))) return rc;
-  if ((rc = qc::check_device_pointer(CALL, "q_dev", q_dev))) return rc;
-  if (gate_dev && (rc = qc::check_device_pointer(CALL, "gate_dev", gate_dev))) return rc;
-  if ((rc = qc::check_device_pointer(CALL, "out_dev", out_dev))) return rc;
-  if ((rc = qc::check_device_pointer(CALL, "workspace", workspace))) return rc;
+  rc = qc::BufferCheck(CALL)
+           .need("the pool", cache->pool)
+           .need("page_table_dev", page_table_dev)
+           .need("len_dev", len_dev)
+           .need("q_dev", q_dev)
+           .maybe("gate_dev", gate_dev)
+           .need("out_dev", out_dev)
+           .need("workspace", workspace)
+           .check();
+  if (rc) return rc;
 
   qc::Kv8AttnArgs a{};
   a.pool = cache->pool;

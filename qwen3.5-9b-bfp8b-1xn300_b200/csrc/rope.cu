@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(RT) rope_kernel(const __grid_constant__ RopeAr
   int p = 0, slice = blockIdx.y;
   while (slice >= a.slices[p]) slice -= a.slices[p++];
   const qc_rope_part& q = a.part[p];
-  const int h0 = slice * a.chunk, h1 = min(h0 + a.chunk, q.n_heads);
+  const int h0 = slice * a.chunk, h1 = min(h0 + a.chunk, int(q.n_heads));
   const int gl = a.gl, j = threadIdx.x & (gl - 1);
   const int64_t r = (int64_t(blockIdx.x) * RT + threadIdx.x) >> a.gl_log2;
   const bool on = r < a.rows && 8 * j < a.dim, turn = on && 8 * j < a.rot;
@@ -282,20 +282,18 @@ extern "C" int qc_rope_apply(const qc_rope* rope, int32_t head_dim, float eps,
   for (int p = 0; p < n_parts; ++p) {
     const qc_rope_part& q = parts[p];
     if (q.n_heads < 1 || q.n_heads > QC_ROPE_MAX_HEADS)
-      return qc::refuse(QC_ERR_ARG, "%s: n_heads %d", CALL, q.n_heads);
+      return qc::refuse(QC_ERR_ARG, "%s: n_heads %lld", CALL, (long long)q.n_heads);
     if ((q.x_ld | q.x_head | q.out_ld | q.out_head) & 7)
       return bad("strides must be multiples of 8 elements");
     if (((uintptr_t)q.x | (uintptr_t)q.out | (uintptr_t)q.norm_w) & 15)
       return bad("x, out and norm_w must be 16-byte aligned");
   }
   if (n_rows == 0) return QC_OK;
-  int rc = qc::check_device_pointer(CALL, "pos_dev", pos_dev);
-  for (int p = 0; p < n_parts && !rc; ++p) {
-    rc = qc::check_device_pointer(CALL, "x", parts[p].x);
-    if (!rc) rc = qc::check_device_pointer(CALL, "out", parts[p].out);
-    if (!rc && parts[p].norm_w) rc = qc::check_device_pointer(CALL, "norm_w", parts[p].norm_w);
-  }
-  if (rc) return rc;
+  qc::BufferCheck buffers(CALL);
+  buffers.need("pos_dev", pos_dev);
+  for (int p = 0; p < n_parts; ++p)
+    buffers.need("x", parts[p].x).need("out", parts[p].out).maybe("norm_w", parts[p].norm_w);
+  if (buffers.check()) return buffers.check();
 
   qc::RopeArgs a{};
   for (int i = 0; i < rope->rot_dim / 2; ++i)
@@ -324,7 +322,7 @@ extern "C" int qc_rope_apply(const qc_rope* rope, int32_t head_dim, float eps,
     int32_t most = 1;
     for (int p = 0; p < n_parts; ++p) {
       norm |= parts[p].norm_w != nullptr;
-      most = std::max(most, parts[p].n_heads);
+      most = std::max(most, int32_t(parts[p].n_heads));
     }
     // A group takes as many of its row's heads as leave WANT threads (two waves of
     // every SM), as each group works out the row's angles again: 2048 rows of 20
@@ -334,7 +332,7 @@ extern "C" int qc_rope_apply(const qc_rope* rope, int32_t head_dim, float eps,
     // 3.1, 128 rows 3.6 and 3.3.
     auto slices = [&](int32_t chunk) {
       int32_t n = 0;
-      for (int p = 0; p < n_parts; ++p) n += a.slices[p] = (parts[p].n_heads + chunk - 1) / chunk;
+      for (int p = 0; p < n_parts; ++p) n += a.slices[p] = (int32_t(parts[p].n_heads) + chunk - 1) / chunk;
       return n;
     };
     constexpr int64_t WANT = 148 * 2048, FEW = 148 * 256;

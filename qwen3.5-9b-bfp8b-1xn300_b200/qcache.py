@@ -77,17 +77,13 @@ class RopePart(C.Structure):
     _fields_ = [
         ("x", C.c_void_p),
         ("out", C.c_void_p),
-        ("norm_w", C.c_void_p),
+        ("n_heads", C.c_int64),
         ("x_ld", C.c_int64),
         ("x_head", C.c_int64),
         ("out_ld", C.c_int64),
         ("out_head", C.c_int64),
-        ("n_heads", C.c_int32),
-        ("reserved", C.c_int32),
+        ("norm_w", C.c_void_p),
     ]
-
-    def __init__(self, x_ptr, out_ptr, n_heads, x_ld, x_head, out_ld, out_head, norm_ptr=0):
-        super().__init__(x_ptr, out_ptr, norm_ptr, x_ld, x_head, out_ld, out_head, n_heads, 0)
 
 
 class Kv8Desc(C.Structure):

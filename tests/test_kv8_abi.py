@@ -70,7 +70,7 @@ def test_rope_init_refuses(qcache):
 
 def test_rope_apply_refuses(qcache):
     rope = qcache.Rope(64)
-    good = dict(x_ptr=16, out_ptr=16, n_heads=4, x_ld=1024, x_head=256, out_ld=1024, out_head=256)
+    good = dict(x=16, out=16, n_heads=4, x_ld=1024, x_head=256, out_ld=1024, out_head=256)
 
     def call(text, dim=256, rows=1, parts=None, eps=1e-6, pos=16, **kw):
         ps = parts if parts is not None else [qcache.RopePart(**{**good, **kw})]
@@ -88,7 +88,7 @@ def test_rope_apply_refuses(qcache):
     call("n_heads", n_heads=16385)
     for s in ("x_ld", "x_head", "out_ld", "out_head"):
         call("multiples of 8", **{s: 1020})
-    for s in ("x_ptr", "out_ptr", "norm_ptr"):
+    for s in ("x", "out", "norm_w"):
         call("aligned", **{s: 24})
     call("pos_dev is null", pos=0)
     rope.apply(256, 0, 0, [qcache.RopePart(**good)])   # no rows: nothing to do
@@ -164,5 +164,5 @@ def test_descriptions_match_the_header(qcache):
     """The ctypes layouts are those of the C structs."""
     assert C.sizeof(qcache.RopeConfig) == 4 * 4 + 5 * 8
     assert C.sizeof(qcache.RopeFrequencies) == 8 + 8 + 128 * 8
-    assert C.sizeof(qcache.RopePart) == 3 * 8 + 4 * 8 + 8
+    assert C.sizeof(qcache.RopePart) == 8 * 8
     assert C.sizeof(qcache.Kv8Desc) == 8 + 4 * 4
