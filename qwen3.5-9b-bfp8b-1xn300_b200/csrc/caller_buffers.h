@@ -64,9 +64,9 @@ class BufferCheck {
 
 // Launch as a programmatic dependent of the kernel before: it may start early and
 // waits (griddepcontrol.wait) before it reads or writes memory.
-template <typename... A>
+template <typename... A, typename... B>
 cudaError_t launch_dependent(void (*k)(A...), dim3 grid, int threads, size_t smem, cudaStream_t s,
-                             const A&... args) {
+                             const B&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads, 1, 1);
@@ -77,7 +77,7 @@ cudaError_t launch_dependent(void (*k)(A...), dim3 grid, int threads, size_t sme
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k, args...);
+  return cudaLaunchKernelEx(&cfg, k, A(args)...);
 }
 
 }  // namespace qc

@@ -476,6 +476,11 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// o 2^(r - m) / l as two factors, the power in two halves: either alone may leave f32.
+__device__ __forceinline__ float2 finish(float m, float l, float r) {
+  const float half = 0.5f * (r - m);
+  return l == 0.0f ? make_float2(0.0f, 0.0f) : make_float2(ex2(half) / l, ex2(r - m - half));
+}
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                         uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile(
@@ -824,10 +829,7 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
       const int h = 2 * t + j;  // o[.][j]: dim g of the 16, o[.][j + 2]: dim g + 8
       if (h >= a.group) continue;
       if (whole) {
-        // o 2^(r - m) / l, the power in two halves: either alone may leave f32
-        const float half = 0.5f * (r[j] - m[j]);
-        const float f1 = l[j] == 0.0f ? 0.0f : ex2(half) / l[j];
-        const float f2 = l[j] == 0.0f ? 0.0f : ex2(r[j] - m[j] - half);
+        const float2 f = finish(m[j], l[j], r[j]);
         const int64_t head = int64_t(kvh) * a.group + h;
         uint16_t* out = a.out + seq * a.out_ld + head * D;
         const uint16_t* gate = a.gate ? a.gate + seq * a.q_ld + head * a.q_head : nullptr;
@@ -836,7 +838,7 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
 #pragma unroll
           for (int k = 0; k < 2; ++k) {
             const int d = 16 * s + 8 * k + g;
-            float y = o[s][j + 2 * k] * f1 * f2;
+            float y = o[s][j + 2 * k] * f.x * f.y;
             if (gate) y *= sigmoid_exact(bf2f(gate[d]));
             out[d] = f2bf(y);
           }
@@ -859,69 +861,92 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
   }
 }
 
-// Merges the records of a split pair: CTA (owner entry, head of the group, CHUNK
-// dims), CHUNK / 4 lanes across the dims and the rest of the 256 threads along
-// the records, which are the owner's and then the first ones of the warps after
-// it.  One pass over the records' heads gives the references and sums, a second
-// adds the o in order.
-template <int D, int CHUNK>
+// ---- merge of the records of split pairs
+//
+// A CTA takes an owner entry, 2^LOG_HG heads of the group and 2^LOG_CHUNK dims (all
+// of them where it takes several heads): a lane for every 4 dims across, the rest
+// of the 256 threads along the records, which are the owner's and then the first
+// ones of the warps after it.  Each thread's first records are loaded with the
+// records' heads, from which the references and sums come; then the o are added in
+// order.  It is latency throughout, so the launch keeps the CTAs to one wave
+// (MERGE_CTAS): few heads have many records each and are spread over many CTAs, many
+// heads share one.  16 x 4096: 256 CTAs 37 us in all, 2048 (32 dims each) 38.8, 4096
+// (16 dims) 54.9; 1 x 131072: 256 CTAs of 16 dims 53.4, 128 of 32 dims 55.9.
+constexpr int MERGE_CTAS = 592;
+
+// l under a reference that moved from m to m1; 0 exactly where no token was met, NaN passes.
+__device__ __forceinline__ float rebase(float l, float m, float m1) {
+  return l == 0.0f || m == m1 ? l : l * ex2(m - m1);
+}
+
+template <int D, int LOG_CHUNK, int LOG_HG>
 __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnArgs a) {
-  constexpr int LANES = CHUNK / 4, SLOTS = 256 / LANES;
-  constexpr int AHEAD = CHUNK == 32 ? 8 : 2;  // of a thread's records, loaded with the heads
-  __shared__ float4 part[SLOTS][LANES];
-  __shared__ float fac[MAX_WARPS];
-  __shared__ float2 top_s[8];
+  constexpr int AHEAD = 5;
+  __shared__ float4 part[256];
+  __shared__ float ref[LOG_HG == 0 ? MAX_WARPS : 1];  // one head: the records' r
+  __shared__ float2 top_s[8];  // per warp: largest m and r of its head's records
   __shared__ float sum_s[8];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int4 own = a.owner[blockIdx.x];
   const int n = own.z;
-  if (n == 0) return;
   // an entry whose warp gave up on a wait is whatever the workspace held: follow it
   // only inside the records and the batch
-  if (n < 0 || n > a.warps || own.w < 0 || own.w / 2 > a.warps - n || own.x < 0 || own.x >= a.n ||
+  if (n <= 0 || n > a.warps || own.w < 0 || own.w / 2 > a.warps - n || own.x < 0 || own.x >= a.n ||
       own.y < 0 || own.y >= a.kv_heads)
     return;
-  const int64_t step = int64_t(a.group) * (D + 4);
-  auto rec = [&](int i) {
-    return a.rec + (i == 0 ? own.w : 2 * (own.w / 2 + i)) * step + h * (D + 4);
+  const auto record = [&](int i, int h) {
+    return a.rec + (int64_t(i == 0 ? own.w : 2 * (own.w / 2 + i)) * a.group + h) * (D + 4);
   };
+  constexpr int QUADS = (1 << LOG_CHUNK) / 4, LANES = QUADS << LOG_HG, SLOTS = 256 / LANES;
+  const int quad = tid % LANES, slot = tid / LANES, hq = quad / QUADS;
+  const int h = (blockIdx.y << LOG_HG) + hq, d = (blockIdx.z << LOG_CHUNK) + quad % QUADS * 4;
+  const bool on = h < a.group;
   const int64_t head = int64_t(own.y) * a.group + h;
-  const int dim = CHUNK * blockIdx.z + tid;
-  float gate = 0.0f;
-  if (a.gate && tid < CHUNK) gate = bf2f(a.gate[own.x * a.q_ld + head * a.q_head + dim]);
-  const int quad = tid % LANES, slot = tid / LANES;
-  const auto values = [&](int i) {
-    return *reinterpret_cast<const float4*>(rec(i) + 4 + CHUNK * blockIdx.z + 4 * quad);
-  };
+  uint2 gate = make_uint2(0, 0);
+  if (a.gate && on && slot == 0)
+    gate = *reinterpret_cast<const uint2*>(a.gate + own.x * a.q_ld + head * a.q_head + d);
   float4 ahead[AHEAD];
+  float at[AHEAD];
 #pragma unroll
   for (int j = 0; j < AHEAD; ++j)
-    if (slot + j * SLOTS < n) ahead[j] = values(slot + j * SLOTS);
+    if (on && slot + j * SLOTS < n) {
+      const float* p = record(slot + j * SLOTS, h);
+      if (LOG_HG > 0) at[j] = p[2];
+      ahead[j] = *reinterpret_cast<const float4*>(p + 4 + d);
+    }
+  // the heads of the records: PER threads, whole warps, for each head
+  constexpr int PER = 256 >> LOG_HG, NW = 8 >> LOG_HG;
+  const int hs = (blockIdx.y << LOG_HG) + tid / PER;
   float m = -INFINITY, r = -INFINITY, l = 0.0f;
-  for (int i = tid; i < n; i += 256) {
-    const float4 s = *reinterpret_cast<const float4*>(rec(i));
-    // l under the running m; it is 0 exactly where a record met no token, NaN passes
+  const int heads_n = hs < a.group ? n : 0;
+#pragma unroll 4
+  for (int i = tid % PER; i < heads_n; i += PER) {
+    const float4 s = *reinterpret_cast<const float4*>(record(i, hs));
     const float m1 = fmaxf(m, s.x);
-    if (s.y != 0.0f) l = l * (l == 0.0f ? 1.0f : ex2(m - m1)) + s.y * (s.x == m1 ? 1.0f : ex2(s.x - m1));
+    l = rebase(l, m, m1) + rebase(s.y, s.x, m1);
     m = m1;
     r = fmaxf(r, s.z);
-    fac[i] = s.y == 0.0f ? -INFINITY : s.z;
+    if (LOG_HG == 0) ref[i] = s.z;
   }
   const float mw = warp_max(m), rw = warp_max(r);
   if (lane == 0) top_s[w] = make_float2(mw, rw);
   __syncthreads();
-  float M = -INFINITY;
-  for (int x = 0; x < 8; ++x) {
-    M = fmaxf(M, top_s[x].x);
-    r = fmaxf(r, top_s[x].y);
-  }
-  l = warp_sum(l == 0.0f || m == M ? l : l * ex2(m - M));
+  const auto top = [&](int first) {
+    float2 t = top_s[first];
+    for (int x = 1; x < NW; ++x) {
+      t.x = fmaxf(t.x, top_s[first + x].x);
+      t.y = fmaxf(t.y, top_s[first + x].y);
+    }
+    return t;
+  };
+  l = warp_sum(rebase(l, m, top(w / NW * NW).x));
   if (lane == 0) sum_s[w] = l;
+  const float2 mr = top(hq * NW);
   float4 o = make_float4(0, 0, 0, 0);
-  const auto add = [&](int i, const float4& x) {
-    const float f = fac[i] == r ? 1.0f : ex2(fac[i] - r);
+  const auto add = [&](float r1, const float4& x) {
+    const float f = r1 == mr.y ? 1.0f : ex2(r1 - mr.y);
     o.x += x.x * f;
     o.y += x.y * f;
     o.z += x.z * f;
@@ -929,25 +954,68 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnArgs a) {
   };
 #pragma unroll
   for (int j = 0; j < AHEAD; ++j)
-    if (slot + j * SLOTS < n) add(slot + j * SLOTS, ahead[j]);
+    if (on && slot + j * SLOTS < n) add(LOG_HG == 0 ? ref[slot + j * SLOTS] : at[j], ahead[j]);
+  const int values_n = on ? n : 0;
 #pragma unroll 4
-  for (int i = slot + AHEAD * SLOTS; i < n; i += SLOTS) add(i, values(i));
-  part[slot][quad] = o;
-  __syncthreads();
-  if (tid < CHUNK) {
-    float y = 0.0f, total = 0.0f;
-    for (int x = 0; x < 8; ++x) total += sum_s[x];
-    for (int s = 0; s < SLOTS; ++s) y += reinterpret_cast<const float*>(part[s])[tid];
-    const float half = 0.5f * (r - M);
-    y = total == 0.0f ? 0.0f : y * (ex2(half) / total) * ex2(r - M - half);
-    if (a.gate) y *= sigmoid_exact(gate);
-    a.out[own.x * a.out_ld + head * D + dim] = f2bf(y);
+  for (int i = slot + AHEAD * SLOTS; i < values_n; i += SLOTS) {
+    const float* p = record(i, h);
+    add(LOG_HG == 0 ? ref[i] : p[2], *reinterpret_cast<const float4*>(p + 4 + d));
   }
+  // the slots of a warp, then those that are left (8 at most)
+#pragma unroll
+  for (int x = LANES; x < 32; x <<= 1) {
+    o.x += __shfl_xor_sync(FULL_MASK, o.x, x);
+    o.y += __shfl_xor_sync(FULL_MASK, o.y, x);
+    o.z += __shfl_xor_sync(FULL_MASK, o.z, x);
+    o.w += __shfl_xor_sync(FULL_MASK, o.w, x);
+  }
+  part[tid] = o;
+  __syncthreads();
+  if (slot != 0 || !on) return;
+  float total = 0.0f;
+  for (int x = 0; x < NW; ++x) total += sum_s[hq * NW + x];
+  constexpr int NEXT = LANES > 32 ? LANES : 32;
+#pragma unroll
+  for (int s = NEXT; s < 256; s += NEXT) {
+    const float4 x = part[s + quad];
+    o.x += x.x;
+    o.y += x.y;
+    o.z += x.z;
+    o.w += x.w;
+  }
+  const float2 f = finish(mr.x, total, mr.y);
+  float y[4] = {o.x * f.x * f.y, o.y * f.x * f.y, o.z * f.x * f.y, o.w * f.x * f.y};
+  if (a.gate) {
+    y[0] *= sigmoid_exact(bf_lo(gate.x));
+    y[1] *= sigmoid_exact(bf_hi(gate.x));
+    y[2] *= sigmoid_exact(bf_lo(gate.y));
+    y[3] *= sigmoid_exact(bf_hi(gate.y));
+  }
+  *reinterpret_cast<uint2*>(a.out + own.x * a.out_ld + head * D + d) =
+      make_uint2(f2bf(y[0]) | uint32_t(f2bf(y[1])) << 16, f2bf(y[2]) | uint32_t(f2bf(y[3])) << 16);
 }
 
 // Workspace: owners of MAX_WARPS warps, then their records.
 int64_t owner_bytes() { return int64_t(MAX_WARPS) * sizeof(int4); }
 int64_t record_bytes(int32_t group, int32_t dim) { return int64_t(group) * (dim + 4) * sizeof(float); }
+
+template <int D, int LOG_CHUNK, int LOG_HG>
+cudaError_t launch_merge_as(const Kv8AttnArgs& a, int entries, cudaStream_t s) {
+  constexpr int HG = 1 << LOG_HG;
+  const int64_t groups = (a.group + HG - 1) / HG;
+  const bool fits = entries * groups * (D >> LOG_CHUNK) <= MERGE_CTAS;
+  if constexpr ((1 << LOG_CHUNK) < D) {
+    if (!fits) return launch_merge_as<D, LOG_CHUNK + 1, LOG_HG>(a, entries, s);
+  } else if constexpr (HG < 8 && HG * D < 1024) {
+    if (!fits && HG < a.group) return launch_merge_as<D, LOG_CHUNK, LOG_HG + 1>(a, entries, s);
+  }
+  return launch_dependent(kv8_merge_kernel<D, LOG_CHUNK, LOG_HG>,
+                          dim3(entries, (unsigned)groups, D >> LOG_CHUNK), 256, 0, s, a);
+}
+template <int D>
+cudaError_t launch_merge(const Kv8AttnArgs& a, int entries, cudaStream_t s) {
+  return launch_merge_as<D, 4, 0>(a, entries, s);
+}
 
 template <int D, bool PAIRED>
 cudaError_t launch_attn(Kv8AttnArgs a, cudaStream_t s) {
@@ -977,10 +1045,7 @@ cudaError_t launch_attn(Kv8AttnArgs a, cudaStream_t s) {
   const int entries = a.by_pair ? int(pairs) : warps;
   e = launch_dependent(kv8_attn_kernel<D, PAIRED>, dim3(grid), 32 * AW, sizeof(AttnSmem<D>), s, a);
   if (e != cudaSuccess) return e;
-  // few heads have many records each: then 32 dims to a CTA, 32 threads along them
-  if (entries * a.group <= 256)
-    return launch_dependent(kv8_merge_kernel<D, 32>, dim3(entries, a.group, D / 32), 256, 0, s, a);
-  return launch_dependent(kv8_merge_kernel<D, D>, dim3(entries, a.group, 1), 256, 0, s, a);
+  return launch_merge<D>(a, entries, s);
 }
 
 int check_cache(const char* call, const qc_kv8_cache* c) {
