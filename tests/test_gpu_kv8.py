@@ -249,6 +249,30 @@ def test_other_pages_and_blocks_keep_their_bytes(qcache):
     qcache.kv8_check()
 
 
+def test_rows_behind_the_last_sequence(qcache):
+    """More rows than the sequences take (a padded batch): those are not read on
+    a write and stay as they were on a read."""
+    pool, model, g = Pool(qcache, 2, 2, 2, 128), Model(2, 2, 128), gen(12)
+    k, v = rows_of(g, 100, 2, 128), rows_of(g, 100, 2, 128)
+    k[60:], v[60:] = math.nan, math.inf
+    # every index array stays referenced until the kernels that read it are done
+    zero, pos, start0, start, back = (i32(x) for x in ([0, 0], [0, 7], [5, 12, 19], [5, 25, 60], [3, 23, 65]))
+    pool.cache.write(pool.table.data_ptr(), 2, zero.data_ptr(), start0.data_ptr(), 2, 100, k.data_ptr(), 256, v.data_ptr(), 256)
+    model.write(0, 0, k[5:12], v[5:12])
+    model.write(1, 0, k[12:19], v[12:19])
+    pool.cache.write(pool.table.data_ptr(), 2, pos.data_ptr(), start.data_ptr(), 2, 100, k.data_ptr(), 256, v.data_ptr(), 256)
+    model.write(0, 0, k[5:25], v[5:25])
+    model.write(1, 7, k[25:60], v[25:60])
+    ko, vo = torch.full_like(k, 7.0), torch.full_like(v, 7.0)
+    pool.cache.read(pool.table.data_ptr(), 2, zero.data_ptr(), back.data_ptr(), 2, 100, ko.data_ptr(), 256, vo.data_ptr(), 256)
+    torch.cuda.synchronize()
+    qcache.kv8_check()
+    for got, w in ((ko, 0), (vo, 1)):
+        equal(got[3:23], model.values(0, 0, 20)[w])
+        equal(got[23:65], model.values(1, 0, 42)[w])
+        assert bool((got[:3] == 7.0).all()) and bool((got[65:] == 7.0).all())
+
+
 def test_pages_behind_four_gigabytes(qcache):
     """Pages whose byte offset passes 32 bits; the pool is not filled, only its
     last and first pages are touched."""
