@@ -450,13 +450,15 @@ struct Kv8AttnArgs {
 
 constexpr int AW = 4;                                    // warps per CTA
 // Blocks of a step, what a warp copies and works on at once (8 KB of codes, and
-// the step's fixed part paid once); steps in flight per warp; CTAs per SM.  Of the
-// shapes that fit an SM's shared memory these were the fastest (us): D 256, 64 x
-// 4096: 8 warps of 3 steps 97.7, 12 of 2 98.6, 9 of 3 124; D 128, 33 ragged: steps
-// of 2 blocks 19.3, of 1 block 22.7; D 64, 64 x 8000: 4 blocks in 12 warps 52.7, in
-// 8 warps 55.8, of 2 blocks 54.5, of 1 block 58.
+// the step's fixed part paid once); steps in flight per warp; CTAs per SM.  16
+// copies of 8 KB in flight per SM are enough and more do harm: the SMs then share
+// the bandwidth unevenly and the equal ranges end far apart.  D 256, 64 x 4096 and 1
+// x 131072 (us): 8 warps of 2 steps 88.8 and 50.6, of 3 steps 96.9 and 56.3; 10 of 2
+// 97.8 and 56.3; 6 of 2 95.6 and 53.2; 4 of 4 105 and 57.  D 128, 32 x 4096: 8 of 2
+// 49.3, of 3 52.1; steps of one block 57.3.  D 64, 64 x 8000: 12 of 2 50.9, 10 of 2
+// 55.6, 8 of 2 65.8 (more arithmetic per byte).
 __host__ __device__ constexpr int step_blocks(int dim) { return 256 / dim; }
-__host__ __device__ constexpr int stages(int dim) { return dim == 64 ? 2 : 3; }
+__host__ __device__ constexpr int stages(int dim) { return 2; }
 __host__ __device__ constexpr int ctas_per_sm(int dim) { return dim == 64 ? 3 : 2; }
 constexpr int MAX_WARPS = 1824;                          // of the grid
 constexpr float LAZY_M = 8.0f, TOP_R = 7.0f, LAZY_R = 15.0f;
@@ -508,6 +510,22 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
+}
+
+// bulk_g2s of bytes that are read once: they leave L2 before what is there already
+// (64 x 4096, three caches in turn: 91.8 -> 88.0 us).
+__device__ __forceinline__ uint64_t streaming_policy() {
+  uint64_t p;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+  return p;
+}
+__device__ __forceinline__ void bulk_g2s_stream(void* dst, const void* src, uint32_t bytes,
+                                                uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint "
+      "[%0], [%1], %2, [%3], %4;" ::"r"(smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar)), "l"(policy)
+      : "memory");
 }
 
 // Tokens of a sequence, as many as its page-table row can name, and their steps.
@@ -635,6 +653,7 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
   c.at = int32_t(begin - start.unit - int64_t(c.head) * c.n);
   Cursor<D> p = c;  // the copies run AS steps ahead
   int put = 0;
+  const uint64_t policy = streaming_policy();
   auto issue = [&]() {  // lane 0: the copy of step p into the next stage
     if (p.unit >= end) return;
     const int32_t block = p.at * GB;
@@ -645,10 +664,11 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
     if (ok) {
       const uint32_t bytes = (tokens + BT - 1) / BT * block_bytes(D);
       mbar_arrive_expect_tx(&sm.full[w][put], bytes);
-      bulk_g2s(sm.stage[w][put],
-               a.pool + ((int64_t(page) * a.kv_heads + p.head) * PAGE_BLOCKS + block % PAGE_BLOCKS) *
-                            block_bytes(D),
-               bytes, &sm.full[w][put]);
+      bulk_g2s_stream(
+          sm.stage[w][put],
+          a.pool + ((int64_t(page) * a.kv_heads + p.head) * PAGE_BLOCKS + block % PAGE_BLOCKS) *
+                       block_bytes(D),
+          bytes, &sm.full[w][put], policy);
     } else {
       record_error(&g_kv8_error, QC_ERR_BOUNDS);
       mbar_arrive(&sm.full[w][put]);
