@@ -846,29 +846,43 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-      const int h = 2 * t + j;  // o[.][j]: dim g of the 16, o[.][j + 2]: dim g + 8
+      // o[.][j]: dim g of the 16 and head 2t + j, o[.][j + 2]: dim g + 8.  PAIRED: both lanes
+      // t and t + 2 have heads 2t, 2t + 1 by now; the first stores the dims g, the other g + 8
+      const int h = PAIRED ? 2 * (t & 1) + j : 2 * t + j;
+      constexpr int EACH = PAIRED ? 1 : 2;  // of the two
+      const int d0 = PAIRED ? 8 * (t >> 1) + g : g;
+      const auto value = [&](int s, int k) {
+        return PAIRED ? (t < 2 ? o[s][j] : o[s][j + 2]) : o[s][j + 2 * k];
+      };
       if (h >= a.group) continue;
       if (whole) {
         const float2 f = finish(m[j], l[j], r[j]);
         const int64_t head = int64_t(kvh) * a.group + h;
-        uint16_t* out = a.out + seq * a.out_ld + head * D;
-        const uint16_t* gate = a.gate ? a.gate + seq * a.q_ld + head * a.q_head : nullptr;
+        uint16_t* out = a.out + seq * a.out_ld + head * D + d0;
+        // the gate's logits all come before the first result is stored
+        uint16_t gate[KS][EACH];
+        if (a.gate) {
+          const uint16_t* from = a.gate + seq * a.q_ld + head * a.q_head + d0;
+#pragma unroll
+          for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int k = 0; k < EACH; ++k) gate[s][k] = from[16 * s + 8 * k];
+        }
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const int d = 16 * s + 8 * k + g;
-            float y = o[s][j + 2 * k] * f.x * f.y;
-            if (gate) y *= sigmoid_exact(bf2f(gate[d]));
-            out[d] = f2bf(y);
+          for (int k = 0; k < EACH; ++k) {
+            float y = value(s, k) * f.x * f.y;
+            if (a.gate) y *= sigmoid_exact(bf2f(gate[s][k]));
+            out[16 * s + 8 * k] = f2bf(y);
           }
       } else {
         float* rec = a.rec + ((int64_t(wid) * 2 + (first ? 0 : 1)) * a.group + h) * (D + 4);
-        if (g == 0) *reinterpret_cast<float4*>(rec) = make_float4(m[j], l[j], r[j], 0.0f);
+        if (d0 == 0) *reinterpret_cast<float4*>(rec) = make_float4(m[j], l[j], r[j], 0.0f);
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) rec[4 + 16 * s + 8 * k + g] = o[s][j + 2 * k];
+          for (int k = 0; k < EACH; ++k) rec[4 + d0 + 16 * s + 8 * k] = value(s, k);
       }
     }
     // the range that a pair starts in says what there is to merge
