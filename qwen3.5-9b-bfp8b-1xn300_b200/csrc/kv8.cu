@@ -433,6 +433,12 @@ __global__ void __launch_bounds__(32 * TW, WRITE ? 4 : 1) kv8_rows_kernel(const 
 // that 22 bits of it count.  Both references move only when a score passes them
 // by 2^8 (m; r starts 2^7 under its largest and moves at 2^15), so most blocks
 // rescale nothing.
+//
+// Bound by memory: 64 sequences of 4096 with 4 heads of 256 (538 MB) 88 us, 6.1 TB/s,
+// 0.93 of the measured copy rate, the merge included.  A block costs a warp 32
+// products of 8 cycles and some 550 other instructions, a third of what the SM could
+// issue meanwhile.  mma.sync and not tcgen05: with 1 to 8 query rows the tensor pipe
+// has little to do, and the codes pass through registers on the way to f16 anyway.
 
 struct Kv8AttnArgs {
   const uint8_t* pool;
@@ -904,7 +910,7 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
 // records' heads, from which the references and sums come; then the o are added in
 // order.  It is latency throughout, so the launch keeps the CTAs to one wave
 // (MERGE_CTAS): few heads have many records each and are spread over many CTAs, many
-// heads share one.  16 x 4096: 256 CTAs 37 us in all, 2048 (32 dims each) 38.8, 4096
+// heads share one.  16 x 4096: 256 CTAs 31.4 us in all, 2048 (32 dims each) 38.8, 4096
 // (16 dims) 54.9; 1 x 131072: 256 CTAs of 16 dims 53.4, 128 of 32 dims 55.9.
 constexpr int MERGE_CTAS = 592;
 
