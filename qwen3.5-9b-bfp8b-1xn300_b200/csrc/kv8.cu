@@ -412,12 +412,13 @@ __global__ void __launch_bounds__(32 * TW, WRITE ? 4 : 1) kv8_rows_kernel(const 
 // out = sum_j 2^(x_j - m) V_j / sum_j 2^(x_j - m), x_j = scale * log2(e) q.K_j,
 // one pass over the blocks with a running maximum.
 //
-// Split.  The blocks of all (sequence, kv head) pairs, counted in order, are cut
-// into one equal contiguous range per warp of the grid.  A warp streams its
-// blocks through its own ring of bulk copies (one of 16 + 32 D bytes a block:
-// scales, K, V) and works on each alone: no barrier joins warps.  A pair that
-// lies whole in one range is finished there; of the others every range writes a
-// record (m, l, r, o), which the combine kernel merges in order.
+// Split.  A step is 8 KB of codes: one block of 256-wide heads, two of 128, four of
+// 64, one bulk copy (a block is scales, K, V).  The steps of all (sequence, kv head)
+// pairs, counted in order, are cut into one equal contiguous range per warp of the
+// grid.  A warp streams its steps through its own ring and works on each alone: no
+// barrier joins warps.  A pair that lies whole in one range is finished there; of
+// the others every range writes a record (m, l, r, o), which the merge kernel adds
+// in order.
 //
 // Products.  S = K q on m16n8k16 f16 with f32 sums: the codes are whole numbers
 // up to 127 and the bf16 queries, scaled by a power of two, are exact in f16, so
