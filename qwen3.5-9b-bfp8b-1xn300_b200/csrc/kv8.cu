@@ -415,10 +415,11 @@ __global__ void __launch_bounds__(32 * TW, WRITE ? 4 : 1) kv8_rows_kernel(const 
 // Split.  A step is 8 KB of codes: one block of 256-wide heads, two of 128, four of
 // 64, one bulk copy (a block is scales, K, V).  The steps of all (sequence, kv head)
 // pairs, counted in order, are cut into one equal contiguous range per warp of the
-// grid.  A warp streams its steps through its own ring and works on each alone: no
-// barrier joins warps.  A pair that lies whole in one range is finished there; of
-// the others every range writes a record (m, l, r, o), which the merge kernel adds
-// in order.
+// grid.  A warp streams its steps through its own ring and works on each alone.  A
+// pair that lies whole in one range is finished there; of the others every range
+// writes a record (m, l, r, o), which the merge kernel adds in order.  Where all
+// ranges of a CTA lie in one pair its warps meet once, at the end, and write one
+// record for the four.
 //
 // Products.  S = K q on m16n8k16 f16 with f32 sums: the codes are whole numbers
 // up to 127 and the bf16 queries, scaled by a power of two, are exact in f16, so
@@ -446,8 +447,9 @@ struct Kv8AttnArgs {
   const int32_t *table, *len;
   const uint16_t *q, *gate;
   uint16_t* out;
-  int4* owner;      // a split pair: sequence, kv head, its number of records, the first of them;
-                    // one entry per pair (by_pair) or for the last pair that each warp starts
+  int4* owner;      // a split pair: its number; 8 * joined CTAs + records before them; records;
+                    // slot of the first.  One entry per pair (by_pair) or for the last pair that
+                    // each warp starts
   float* rec;       // [warps][2][group][D + 4]: m, l, r, unused, o
   int64_t q_ld, q_head, out_ld;
   float scale;      // scale * log2(e)
@@ -477,6 +479,7 @@ struct AttnSmem {
   alignas(8) uint64_t full[AW][AS];
   int32_t valid[AW][AS];                                 // tokens of the step; 0: nothing was copied
   int64_t sums[AW];
+  float m[AW][8], l[AW][8], r[AW][8];  // of a joined CTA's warps
   struct { int64_t unit; int32_t seq, n, len; } start[AW];
 };
 
@@ -484,6 +487,10 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// l under a reference that moved from m to m1; 0 exactly where no token was met, NaN passes.
+__device__ __forceinline__ float rebase(float l, float m, float m1) {
+  return l == 0.0f || m == m1 ? l : l * ex2(m - m1);
 }
 // o 2^(r - m) / l as two factors, the power in two halves: either alone may leave f32.
 __device__ __forceinline__ float2 finish(float m, float l, float r) {
@@ -602,9 +609,17 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  const int warps = gridDim.x * AW, wid = w * gridDim.x + blockIdx.x;
+  const int warps = gridDim.x * AW;
   int64_t total, per;
-  const auto share = [&]() { per = max(quotient(total + warps - 1, warps), int64_t(1)); };
+  bool spread;
+  const auto share = [&]() {
+    per = max(quotient(total + warps - 1, warps), int64_t(1));
+    // ranges side by side are one CTA's, so that it can join them; when there is at most
+    // one step for each warp and few for a pair (1 x 1024: 8.5 us, joined 9.1; with 313
+    // steps in one pair 8.3 and 7.3) they go to different SMs
+    spread = total <= warps && total <= int64_t(128) * a.n * a.kv_heads;
+  };
+  const auto range_of = [&](int x) { return spread ? x * int(gridDim.x) + int(blockIdx.x) : int(blockIdx.x) * AW + x; };
   struct { int64_t unit; int32_t seq, n, len; } start;  // the sequence this warp starts in, its first unit
   if (a.n <= 32) {  // a sequence per lane, every warp for itself
     const int32_t len = seq_len(a, min(lane, a.n - 1));
@@ -617,7 +632,7 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
     }
     total = __shfl_sync(FULL_MASK, upto, 31) * a.kv_heads;
     share();
-    const int in = min(__popc(__ballot_sync(FULL_MASK, upto * a.kv_heads <= wid * per)), 31);
+    const int in = min(__popc(__ballot_sync(FULL_MASK, upto * a.kv_heads <= range_of(w) * per)), 31);
     start.unit = __shfl_sync(FULL_MASK, upto - steps, in) * a.kv_heads;
     start.seq = in;
     start.n = __shfl_sync(FULL_MASK, steps, in);
@@ -629,7 +644,7 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
     total *= a.kv_heads;
     share();
     for (int x = 0; x < AW; ++x) {
-      const int64_t u = (int64_t(x) * gridDim.x + blockIdx.x) * per;  // warp x's first step
+      const int64_t u = range_of(x) * per;  // warp x's first step
       if (u >= before * a.kv_heads && u < (before + mine) * a.kv_heads) {
         int64_t at = before;
         int i = tid * ((a.n + 32 * AW - 1) / (32 * AW));
@@ -644,6 +659,7 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
     start.n = sm.start[w].n;
     start.len = sm.start[w].len;
   }
+  const int wid = range_of(w);
   const int64_t begin = wid * per, end = min(begin + per, total);
   if (lane == 0 && !a.by_pair) a.owner[wid] = make_int4(0, 0, 0, 0);
   if (begin >= end) {
@@ -658,6 +674,9 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
   c.len = start.len;
   c.head = int32_t(quotient(begin - start.unit, c.n));
   c.at = int32_t(begin - start.unit - int64_t(c.head) * c.n);
+  // whether the CTA's ranges, none of them empty, lie in one pair: the same for its warps
+  const int64_t u0 = int64_t(blockIdx.x) * AW * per, pair0 = begin - c.at;
+  const bool joined = !spread && u0 >= pair0 && min(u0 + AW * per, total) <= pair0 + c.n && u0 + (AW - 1) * per < total;
   Cursor<D> p = c;  // the copies run AS steps ahead
   int put = 0;
   const uint64_t policy = streaming_policy();
@@ -703,8 +722,8 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
 
   int get = 0;
   uint32_t parity = 0;
-  bool first = true;
-  while (c.unit < end) {
+  bool first = true, dead = false;
+  while (c.unit < end && !dead) {
     // ---- the pair's queries, as operand columns: column n is head n (PAIRED: n % 4)
     const int32_t from = c.at;
     uint32_t qf[KS][2];
@@ -743,7 +762,9 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
           const int x = get + s < AS ? get + s : get + s - AS;
           if (c.unit + s < end) mbar_wait(&sm.full[w][x], get + s < AS ? parity : parity ^ 1, nullptr);
         }
-        return;
+        if (!joined) return;
+        dead = true;  // the others of the CTA wait for this warp
+        break;
       }
       const int valid = sm.valid[w][get];
       const uint8_t* step = sm.stage[w][get];
@@ -851,8 +872,69 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[s][j] += __shfl_xor_sync(FULL_MASK, o[s][j], 2);
     }
+    if (joined) {
+      // every copy of the CTA has landed and been read by the time that its warps meet:
+      // each leaves its sums in its own ring, [dim][two heads], and its references
+      constexpr int HP = PAIRED ? 2 : 4;  // pairs of heads
+      float2* mine = reinterpret_cast<float2*>(sm.stage[w]);
+      __syncwarp();
+      if (t < HP) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+          mine[(16 * s + g) * HP + t] = make_float2(o[s][0], o[s][1]);
+          mine[(16 * s + 8 + g) * HP + t] = make_float2(o[s][2], o[s][3]);
+        }
+        if (g == 0) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            sm.m[w][2 * t + j] = m[j];
+            sm.l[w][2 * t + j] = l[j];
+            sm.r[w][2 * t + j] = r[j];
+          }
+        }
+      }
+      __syncthreads();
+      const int hp = tid % HP;
+      float M[2], L[2], R[2], f[AW][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        M[j] = R[j] = -INFINITY;
+        L[j] = 0.0f;
+#pragma unroll
+        for (int x = 0; x < AW; ++x) {
+          M[j] = fmaxf(M[j], sm.m[x][2 * hp + j]);
+          R[j] = fmaxf(R[j], sm.r[x][2 * hp + j]);
+        }
+#pragma unroll
+        for (int x = 0; x < AW; ++x) {
+          L[j] += rebase(sm.l[x][2 * hp + j], sm.m[x][2 * hp + j], M[j]);
+          const float r1 = sm.r[x][2 * hp + j];
+          f[x][j] = r1 == R[j] ? 1.0f : ex2(r1 - R[j]);
+        }
+      }
+      float* rec = a.rec + (int64_t(blockIdx.x) * AW * 2 * a.group + 2 * hp) * (D + 4);
+      const bool two = 2 * hp + 1 < a.group;
+#pragma unroll
+      for (int i = 0; i < D * HP / (32 * AW); ++i) {
+        const int item = i * 32 * AW + tid, d = item / HP;
+        float2 y = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int x = 0; x < AW; ++x) {
+          const float2 z = reinterpret_cast<const float2*>(sm.stage[x])[item];
+          y.x += z.x * f[x][0];
+          y.y += z.y * f[x][1];
+        }
+        if (2 * hp < a.group) rec[4 + d] = y.x;
+        if (two) rec[D + 8 + d] = y.y;
+      }
+      if (tid < HP) {
+        if (2 * hp < a.group) *reinterpret_cast<float4*>(rec) = make_float4(M[0], L[0], R[0], 0.0f);
+        if (two) *reinterpret_cast<float4*>(rec + D + 4) = make_float4(M[1], L[1], R[1], 0.0f);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
+      if (joined) break;
       // o[.][j]: dim g of the 16 and head 2t + j, o[.][j + 2]: dim g + 8.  PAIRED: both lanes
       // t and t + 2 have heads 2t, 2t + 1 by now; the first stores the dims g, the other g + 8
       const int h = PAIRED ? 2 * (t & 1) + j : 2 * t + j;
@@ -893,10 +975,20 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
       }
     }
     // the range that a pair starts in says what there is to merge
-    if (lane == 0 && from == 0 && (!done || a.by_pair)) {
-      const int64_t last = quotient(pair_end - 1, per);
-      a.owner[a.by_pair ? seq * a.kv_heads + kvh : wid] =
-          make_int4(seq, kvh, done ? 0 : int(last) - wid + 1, 2 * wid + (first ? 0 : 1));
+    if (lane == 0 && from == 0 && (!done || joined || a.by_pair)) {
+      const int64_t number = int64_t(seq) * a.kv_heads + kvh;
+      int4 own = make_int4(int(number), 0, 0, 2 * wid + (first ? 0 : 1));
+      if (!whole || joined) {
+        // its warps; the CTAs that it fills, from cta0 on; the records before them
+        const int n = int(quotient(pair_end - 1, per)) - wid + 1;
+        const int cta0 = (first ? wid + AW - 1 : wid + AW) / AW;
+        const int64_t full = pair_end == total ? quotient(total + per - 1, per) / AW
+                                               : quotient(pair_end, AW * per);
+        const int ctas = spread ? 0 : int(max(full - cta0, int64_t(0))), before = ctas ? cta0 * AW - wid : 0;
+        own.y = 8 * ctas + before;
+        own.z = n - (AW - 1) * ctas;
+      }
+      a.owner[a.by_pair ? number : wid] = own;
     }
     first = false;
   }
@@ -907,18 +999,13 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
 // A CTA takes an owner entry, 2^LOG_HG heads of the group and 2^LOG_CHUNK dims (all
 // of them where it takes several heads): a lane for every 4 dims across, the rest
 // of the 256 threads along the records, which are the owner's and then the first
-// ones of the warps after it.  Each thread's first records are loaded with the
+// ones of the warps after it (of a joined CTA's its one).  Each thread's first records are loaded with the
 // records' heads, from which the references and sums come; then the o are added in
 // order.  It is latency throughout, so the launch keeps the CTAs to one wave
 // (MERGE_CTAS): few heads have many records each and are spread over many CTAs, many
 // heads share one.  16 x 4096: 256 CTAs 31.4 us in all, 2048 (32 dims each) 38.8, 4096
 // (16 dims) 54.9; 1 x 131072: 256 CTAs of 16 dims 53.4, 128 of 32 dims 55.9.
 constexpr int MERGE_CTAS = 592;
-
-// l under a reference that moved from m to m1; 0 exactly where no token was met, NaN passes.
-__device__ __forceinline__ float rebase(float l, float m, float m1) {
-  return l == 0.0f || m == m1 ? l : l * ex2(m - m1);
-}
 
 template <int D, int LOG_CHUNK, int LOG_HG>
 __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnArgs a) {
@@ -931,23 +1018,26 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnArgs a) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int4 own = a.owner[blockIdx.x];
-  const int n = own.z;
+  const int n = own.z, ctas = own.y >> 3, before = own.y & 7, wid0 = own.w >> 1;
   // an entry whose warp gave up on a wait is whatever the workspace held: follow it
   // only inside the records and the batch
-  if (n <= 0 || n > a.warps || own.w < 0 || own.w / 2 > a.warps - n || own.x < 0 || own.x >= a.n ||
-      own.y < 0 || own.y >= a.kv_heads)
+  if (n <= 0 || n > a.warps || own.y < 0 || ctas > n || before > AW || own.w < 0 ||
+      wid0 > a.warps - n - (AW - 1) * ctas || own.x < 0 || own.x >= a.n * a.kv_heads)
     return;
+  const int seq = own.x / a.kv_heads, kvh = own.x - seq * a.kv_heads;
+  // record i: the owner's, then a warp's each, the joined CTAs', again a warp's each
   const auto record = [&](int i, int h) {
-    return a.rec + (int64_t(i == 0 ? own.w : 2 * (own.w / 2 + i)) * a.group + h) * (D + 4);
+    const int skip = (AW - 1) * min(max(i - before, 0), ctas);
+    return a.rec + (int64_t(i == 0 ? own.w : 2 * (wid0 + i + skip)) * a.group + h) * (D + 4);
   };
   constexpr int QUADS = (1 << LOG_CHUNK) / 4, LANES = QUADS << LOG_HG, SLOTS = 256 / LANES;
   const int quad = tid % LANES, slot = tid / LANES, hq = quad / QUADS;
   const int h = (blockIdx.y << LOG_HG) + hq, d = (blockIdx.z << LOG_CHUNK) + quad % QUADS * 4;
   const bool on = h < a.group;
-  const int64_t head = int64_t(own.y) * a.group + h;
+  const int64_t head = int64_t(kvh) * a.group + h;
   uint2 gate = make_uint2(0, 0);
   if (a.gate && on && slot == 0)
-    gate = *reinterpret_cast<const uint2*>(a.gate + own.x * a.q_ld + head * a.q_head + d);
+    gate = *reinterpret_cast<const uint2*>(a.gate + seq * a.q_ld + head * a.q_head + d);
   float4 ahead[AHEAD];
   float at[AHEAD];
 #pragma unroll
@@ -1032,7 +1122,7 @@ __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnArgs a) {
     y[2] *= sigmoid_exact(bf_lo(gate.y));
     y[3] *= sigmoid_exact(bf_hi(gate.y));
   }
-  *reinterpret_cast<uint2*>(a.out + own.x * a.out_ld + head * D + d) =
+  *reinterpret_cast<uint2*>(a.out + seq * a.out_ld + head * D + d) =
       make_uint2(f2bf(y[0]) | uint32_t(f2bf(y[1])) << 16, f2bf(y[2]) | uint32_t(f2bf(y[3])) << 16);
 }
 
