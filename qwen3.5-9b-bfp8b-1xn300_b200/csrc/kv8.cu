@@ -134,7 +134,11 @@ __device__ __forceinline__ uint32_t storable2(uint32_t pair) {
 // store per token, all in flight at once.  Rows and codes meet in 16 D bytes of
 // shared memory per tile, which stand in the pool's order (16-byte chunks, D / 32
 // groups of 32) with each group's chunks swapped about by its number, so that
-// neither side's accesses share banks.  Bound by memory.
+// neither side's accesses share banks.  Bound by memory: 65536 tokens of 8 heads of
+// 128 (403 MB) written in 70 us, 5.75 TB/s, 0.88 of the measured copy rate, read in
+// 65 us, 0.95.  The first form, a thread per 16 bytes of the pool with 2-byte loads
+// of V, took 222 us each.  A write holds its 16 rows in registers, which leaves 16
+// warps per SM; 20 of them spilled (164 us for both instead of 151 then).
 template <int D, bool WRITE>
 __global__ void __launch_bounds__(32 * TW, WRITE ? 4 : 1) kv8_rows_kernel(const Kv8RowsArgs a) {
   constexpr int LPT = D / 8, TILES = 32 / LPT;  // lanes per tile, tiles per warp
