@@ -101,8 +101,7 @@ int qc_kv8_read(const qc_kv8_cache* cache, const int32_t* page_table_dev, int32_
  * workspace: at least qc_kv8_attn_workspace_bytes bytes of device memory, 16-
  * byte aligned, for this call alone while it runs; its contents do not matter.
  * Products of queries and codes are exact and sums are kept in f32; the softmax
- * weights enter the second product with 22 bits for groups of up to 4 query heads
- * per KV head, with 11 bits for larger ones.  The result rounds to bf16 once.  It
+ * weights enter the second product with 22 bits.  The result rounds to bf16 once.  It
  * depends on the shapes and values alone: the same bits on every call.  A NaN or
  * infinity in q makes its head's row NaN. */
 int64_t qc_kv8_attn_workspace_bytes(const qc_kv8_cache* cache, int32_t n, int32_t n_head);

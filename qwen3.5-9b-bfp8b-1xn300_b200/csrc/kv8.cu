@@ -434,11 +434,12 @@ __global__ void __launch_bounds__(32 * TW, WRITE ? 4 : 1) kv8_rows_kernel(const 
 //
 // The weights of the second product carry V's scale: w = 2^(x + log2 sv - r)
 // with a running reference r of its own, so blocks of very different scales
-// keep their precision (l has no part in it).  w stands in f16, at most 2^15;
-// groups of up to 4 heads use the product's other 4 columns for w - f16(w), so
-// that 22 bits of it count.  Both references move only when a score passes them
-// by 2^8 (m; r starts 2^7 under its largest and moves at 2^15), so most blocks
-// rescale nothing.
+// keep their precision (l has no part in it).  w stands in f16, at most 2^15, and
+// w - f16(w) beside it, so that 22 bits of it count: in the product's other 4
+// columns for groups of up to 4 heads, in a second product for larger ones (64 x
+// 4096 with 6 heads of 128 to a KV head 86.5 -> 87.8 us, 33 sequences of up to 8191
+// 20.0 -> 21.0).  Both references move only when a score passes them by 2^8 (m; r
+// starts 2^7 under its largest and moves at 2^15), so most blocks rescale nothing.
 //
 // Bound by memory: 64 sequences of 4096 with 4 heads of 256 (538 MB) 88 us, 6.1 TB/s,
 // 0.93 of the measured copy rate, the merge included.  A block costs a warp 32
@@ -841,13 +842,25 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
         }
         const uint32_t b0 = transpose8(pack_f16(y[0], y[1]));
         const uint32_t b1 = transpose8(pack_f16(y[2], y[3]));
+        uint32_t r0 = 0, r1 = 0;  // the rest, where it has no columns of its own
+        if (!PAIRED) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[j] -= __half2float(__float2half_rn(y[j]));
+          r0 = transpose8(pack_f16(y[0], y[1]));
+          r1 = transpose8(pack_f16(y[2], y[3]));
+        }
         const uint4* vc =
             reinterpret_cast<const uint4*>(step + b * block_bytes(D) + HEAD_BYTES) + D + lane;
 #pragma unroll
         for (int i = 0; i < KS / 2; ++i) {
           const uint4 v = vc[32 * i];
-          mma_f16(o[2 * i], codes_lo(v.x), codes_lo(v.y), codes_hi(v.x), codes_hi(v.y), b0, b1);
-          mma_f16(o[2 * i + 1], codes_lo(v.z), codes_lo(v.w), codes_hi(v.z), codes_hi(v.w), b0, b1);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t x0 = half ? v.z : v.x, x1 = half ? v.w : v.y;
+            const uint32_t a0 = codes_lo(x0), a1 = codes_lo(x1), a2 = codes_hi(x0), a3 = codes_hi(x1);
+            mma_f16(o[2 * i + half], a0, a1, a2, a3, b0, b1);
+            if (!PAIRED) mma_f16(o[2 * i + half], a0, a1, a2, a3, r0, r1);
+          }
         }
       }
       __syncwarp();  // every lane has read the stage
@@ -953,20 +966,19 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
         const int64_t head = int64_t(kvh) * a.group + h;
         uint16_t* out = a.out + seq * a.out_ld + head * D + d0;
         // the gate's logits all come before the first result is stored
-        uint16_t gate[KS][EACH];
+        uint32_t gate[KS];  // of both dims
         if (a.gate) {
           const uint16_t* from = a.gate + seq * a.q_ld + head * a.q_head + d0;
 #pragma unroll
           for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int k = 0; k < EACH; ++k) gate[s][k] = from[16 * s + 8 * k];
+            gate[s] = from[16 * s] | (PAIRED ? 0u : uint32_t(from[16 * s + 8]) << 16);
         }
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
           for (int k = 0; k < EACH; ++k) {
             float y = value(s, k) * f.x * f.y;
-            if (a.gate) y *= sigmoid_exact(bf2f(gate[s][k]));
+            if (a.gate) y *= sigmoid_exact(k ? bf_hi(gate[s]) : bf_lo(gate[s]));
             out[16 * s + 8 * k] = f2bf(y);
           }
       } else {

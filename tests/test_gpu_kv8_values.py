@@ -1,0 +1,62 @@
+"""The 8-bit cache's attention where its arithmetic is tight: weights that cancel,
+whatever the number of query heads to a KV head.
+
+The results are compared with the softmax in 64 bits over the values read back.
+Tolerance per element, worked out before the first run, with A = sum p |v|, S =
+scale * sum |q_d k_d| at its largest over the tokens, N = len / 16 blocks:
+  - the bf16 result rounds once: 2^-8 |y| (half a step);
+  - a weight w enters the second product as two f16, w and the rest: the rest is at
+    most 2^-11 w and off by 2^-12 of itself, under 2^-22 w in all;
+  - f32 sums of D products of q and k: (D + 8) 2^-23 S on a score, so as much on
+    the weight; the exponential and its argument 8 * 2^-23 (1 + S);
+  - f32 sums over N + 16 blocks' weights and products: (N + 16) 2^-23 A, twice
+    (numerator and denominator);
+  - f16 ends at 2^-24, so a weight is off by up to 2^-25 however small it is, while
+    the largest is 2^7 or more: len 2^-31 max_j(p_j u_j), u_j the largest |v| of token
+    j's block.
+"""
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+
+from test_gpu_kv8 import Pool, attend, gen, rows_of  # noqa: E402
+
+
+def check(got, q, k, v, scale):
+    """One sequence's rows got [heads][dim] against 64 bits over k, v [len][kv][dim]."""
+    heads, dim = q.shape
+    kv = k.shape[1]
+    qi = q.double().unflatten(0, (kv, heads // kv))
+    kk, vv = k.double().permute(1, 2, 0), v.double().transpose(0, 1)
+    p = torch.softmax(qi @ kk * scale, -1)
+    y, a = p @ vv, p @ vv.abs()
+    s = (qi.abs() @ kk.abs() * abs(scale)).amax(-1, keepdim=True)
+    n = len(k) / 16
+    f = 2.0 ** -22 + (dim + 8) * 2.0 ** -23 * s + 8 * 2.0 ** -23 * (1 + s)
+    u = torch.cat([b.abs().amax((1, 2), keepdim=True).expand(-1, b.shape[1], 1) for b in vv.split(16, 1)], 1)
+    tol = a * (f + 2 * (n + 16) * 2.0 ** -23) + len(k) * 2.0 ** -31 * (p * u.transpose(1, 2)).amax(-1, keepdim=True)
+    tol = tol + (y.abs() + tol) * 2.0 ** -8 + 1e-38
+    err = (got.double().unflatten(0, (kv, heads // kv)) - y).abs()
+    assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.parametrize("kv,group,dim", [(2, 1, 64), (1, 4, 256), (3, 5, 128), (2, 6, 128), (1, 6, 256), (1, 7, 64), (2, 8, 64),
+                                          (1, 8, 256)])
+def test_weights_that_cancel(qcache, kv, group, dim):
+    """Values of opposite sign under nearly equal weights: what is left of them is
+    far below the sum of their magnitudes, so that weights of 11 bits would show."""
+    g = gen(100 * group + dim)
+    lens = [2, 3, 17, 40, 301, 5000]
+    pool = Pool(qcache, len(lens), 79, kv, dim)
+    sign = [torch.tensor([(-1.0) ** j for j in range(n)], device="cuda")[:, None, None] for n in lens]
+    v = torch.cat([s * torch.randn(1, kv, dim, generator=g, device="cuda") for s in sign]).bfloat16()
+    k = rows_of(g, sum(lens), kv, dim)
+    q = rows_of(g, len(lens), kv * group, dim, 0.02)
+    pool.write([0] * len(lens), lens, k, v)
+    k, v = pool.read([0] * len(lens), lens)
+    got = attend(qcache, pool.cache, pool.table, lens, q)
+    for i, (ki, vi) in enumerate(zip(k.split(lens), v.split(lens))):
+        check(got[i], q[i], ki, vi, dim ** -0.5)
+    qcache.kv8_check()
