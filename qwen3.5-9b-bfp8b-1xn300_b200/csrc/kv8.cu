@@ -12,6 +12,7 @@
 // so that a lane's four bytes of one token (K) or of one dim (V) are contiguous.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include <cuda_fp16.h>
 
@@ -457,7 +458,8 @@ struct Kv8AttnArgs {
                     // each warp starts
   float* rec;       // [warps][2][group][D + 4]: m, l, r, unused, o
   int64_t q_ld, q_head, out_ld;
-  float scale;      // scale * log2(e)
+  float scale;      // scale * log2(e) = scale * 2^scale_exp, scale in [0.5, 1)
+  int32_t scale_exp;
   int32_t n_pages, pt_stride, kv_heads, group, n;
   int32_t by_pair, warps;
 };
@@ -732,7 +734,7 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
     // ---- the pair's queries, as operand columns: column n is head n (PAIRED: n % 4)
     const int32_t from = c.at;
     uint32_t qf[KS][2];
-    float qs[2];  // what a column's products count for: scale log2(e) / the power of two in q
+    float qs[2], qt[2];  // a column's products count for qs * qt
     {
       uint32_t top = 0;
 #pragma unroll
@@ -740,10 +742,15 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
       top = max(top & 0xffffu, top >> 16);
       top = max(top, __shfl_xor_sync(FULL_MASK, top, 1));
       top = max(top, __shfl_xor_sync(FULL_MASK, top, 2));
-      // up * 2^e: the largest value into [2^13, 2^14), so that values 2^-37 of it stay exact
-      const int e = max(int(top >> 7) - 127 - 13, -126);
+      // q / 2^e: the largest value into [2^13, 2^14), so that values 2^-37 of it stay exact.
+      // The products count for scale * 2^at, one factor of which is applied before K's scale
+      // and one after it, so that a score whose factors are far apart (q near 2^120, K near
+      // 2^-120) leaves f32 at no step.
+      const int e = max(int(top >> 7) - 127 - 13, -126), at = e + a.scale_exp;
+      const int late = at > 0 ? at / 2 : at < -100 ? -64 : 0;
       const float up = __uint_as_float(uint32_t(127 - e) << 23);
-      float back = a.scale * __uint_as_float(uint32_t(127 + e) << 23);
+      const float after = __uint_as_float(uint32_t(127 + late) << 23);
+      float back = a.scale * __uint_as_float(uint32_t(max(127 + at - late, 1)) << 23);
       if (top >= 0x7f80u) back = __uint_as_float(0x7fc00000u);  // the whole row is NaN
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
@@ -753,6 +760,8 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
       }
       qs[0] = __shfl_sync(FULL_MASK, back, 8 * t);
       qs[1] = __shfl_sync(FULL_MASK, back, 8 * t + 4);
+      qt[0] = __shfl_sync(FULL_MASK, after, 8 * t);
+      qt[1] = __shfl_sync(FULL_MASK, after, 8 * t + 4);
     }
     float m[2] = {-INFINITY, -INFINITY}, r[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
     float o[KS][4];
@@ -796,7 +805,7 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
           lsv[b] = float(int((__float_as_uint(sc.y) >> 23) & 0xffu) - 127);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            x[b][j] = (acc[0][j] + acc[1][j]) * qs[j & 1] * sc.x;
+            x[b][j] = (acc[0][j] + acc[1][j]) * qs[j & 1] * sc.x * qt[j & 1];
             if (b * BT + rho + (j & 2) >= valid) x[b][j] = -INFINITY;
             top[j & 1] = fmaxf(top[j & 1], x[b][j]);
             top_v[j & 1] = fmaxf(top_v[j & 1], x[b][j] + lsv[b]);
@@ -1364,7 +1373,8 @@ extern "C" int qc_kv8_attn_decode(const qc_kv8_cache* cache, const int32_t* page
   a.out_ld = out_ld;
   a.owner = static_cast<int4*>(workspace);
   a.rec = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + qc::owner_bytes());
-  a.scale = scale * 1.44269504088896340736f;  // log2(e): the weights are powers of two
+  a.scale = std::frexp(scale * 1.44269504088896340736f, &a.scale_exp);  // log2(e): the weights are powers of two
+  if (!std::isfinite(a.scale)) a.scale_exp = 0;
   a.n_pages = cache->n_pages;
   a.pt_stride = pt_stride;
   a.kv_heads = kvh;

@@ -60,3 +60,23 @@ def test_weights_that_cancel(qcache, kv, group, dim):
     for i, (ki, vi) in enumerate(zip(k.split(lens), v.split(lens))):
         check(got[i], q[i], ki, vi, dim ** -0.5)
     qcache.kv8_check()
+
+
+@pytest.mark.parametrize("a,b,c", [(0, 0, 0), (120, -118, -2), (115, -119, 4), (122, -120, 2), (124, -122, 2), (-126, 124, 2), (-120, 118, 2), (-60, -60, 120),
+                                   (100, 30, -126), (30, 100, -127), (-110, -10, 120)])
+@pytest.mark.parametrize("group,dim", [(4, 256), (8, 128), (2, 64)])
+def test_moderate_scores_of_extreme_factors(qcache, group, dim, a, b, c):
+    """Queries near 2^a, keys near 2^b and a scale near 2^c whose product is moderate:
+    no step on the way to a score leaves f32, whichever of them is large."""
+    g = gen(200 + a)
+    lens = [1, 20, 700]
+    pool = Pool(qcache, 3, 11, 2, dim)
+    k, v = (rows_of(g, sum(lens), 2, dim).double() * 2.0 ** b).bfloat16(), rows_of(g, sum(lens), 2, dim)
+    q = (rows_of(g, 3, 2 * group, dim).double() * 2.0 ** a).bfloat16()
+    scale = dim ** -0.5 * 2.0 ** c
+    pool.write([0] * 3, lens, k, v)
+    k, v = pool.read([0] * 3, lens)
+    got = attend(qcache, pool.cache, pool.table, lens, q, scale=scale)
+    for i, (ki, vi) in enumerate(zip(k.split(lens), v.split(lens))):
+        check(got[i], q[i], ki, vi, scale)
+    qcache.kv8_check()
