@@ -47,6 +47,36 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// The norm's factor 1 / sqrt(mean(y^2) + eps) of a group's head, of which this lane has
+// 8 dims; all lanes of the warp call it.  Where the squares leave f32 (values beyond
+// 1.8e19, or all below 3e-14 with as small an eps) y is first brought to about 1 by a
+// power of two, exactly but for what is 2^-126 of the head's largest value.  The vote on
+// that costs 2048 rows of 20 heads of 256 0.6 of 11.8 us; one vote for four heads, or
+// a loop of their own for such heads, costs as much or more, in registers.
+__device__ __forceinline__ float norm_factor(const RopeArgs& a, float (&y)[8]) {
+  const auto mean = [&](float eps) {
+    float ss = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
+    for (int m = a.gl >> 1; m; m >>= 1) ss += __shfl_xor_sync(FULL_MASK, ss, m);
+    return ss * a.inv_dim + eps;
+  };
+  float v = mean(a.eps);
+  const bool odd = !(v >= 0x1p-90f && v < INFINITY);
+  if (__any_sync(FULL_MASK, odd)) {
+    float top = sqrtf(a.eps);  // eps * down^2 must not leave f32 either
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(y[e]));
+    for (int m = a.gl >> 1; m; m >>= 1) top = fmaxf(top, __shfl_xor_sync(FULL_MASK, top, m));
+    const int at = int(__float_as_uint(top) >> 23);  // 255: an infinity, the sum shows it
+    const float down = odd && top > 0.0f && at < 255 ? __uint_as_float(uint32_t(max(254 - at, 1)) << 23) : 1.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] *= down;
+    v = mean(a.eps * down * down);
+  }
+  return rsqrtf(v);
+}
+
 // rot_dim a multiple of 8.  gl lanes take a row's heads h0 .. h1-1 of one part
 // (blockIdx.y); lane j holds pairs 4j .. 4j+3 for j < rot / 8 — in the half
 // layout two runs of 4 dims, 4j and rot/2 + 4j, in the interleaved one 8 dims in
@@ -103,16 +133,10 @@ __global__ void __launch_bounds__(RT) rope_kernel(const __grid_constant__ RopeAr
     for (int u = 0; u < RU; ++u) {
       float y[8];
       unpack8(x[u], y);
-      if (NORM) {
-        float ss = 0.0f;
+      if (norm) {
+        const float rms = norm_factor(a, y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(y[e], y[e], ss);
-        for (int m = gl >> 1; m; m >>= 1) ss += __shfl_xor_sync(FULL_MASK, ss, m);
-        if (norm) {
-          const float rms = rsqrtf(ss * a.inv_dim + a.eps);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = y[e] * rms * w[e];
-        }
+        for (int e = 0; e < 8; ++e) y[e] = y[e] * rms * w[e];
       }
       if (turn) {
 #pragma unroll
@@ -162,11 +186,7 @@ __global__ void __launch_bounds__(RT) rope_any_kernel(const __grid_constant__ Ro
         float x[8] = {};
         if (on) unpack8(*reinterpret_cast<const uint4*>(q.x + r * q.x_ld + h * q.x_head + sub * 8), x);
         if (q.norm_w) {
-          float ss = 0.0f;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-          for (int m = gl >> 1; m; m >>= 1) ss += __shfl_xor_sync(FULL_MASK, ss, m);
-          const float rms = rsqrtf(ss * a.inv_dim + a.eps);
+          const float rms = norm_factor(a, x);
           if (on) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) x[e] = x[e] * rms * q.norm_w[sub * 8 + e];
