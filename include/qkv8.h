@@ -112,9 +112,12 @@ int qc_kv8_attn_decode(const qc_kv8_cache* cache, const int32_t* page_table_dev,
                        const uint16_t* gate_dev, float scale, uint16_t* out_dev, int64_t out_ld,
                        void* workspace, int64_t workspace_bytes, qc_stream stream);
 
-/* Synchronises `stream` and returns the first error that the kernels of this
- * header have recorded on the current device since the last call (QC_ERR_BOUNDS,
- * QC_ERR_TIMEOUT), clearing it. */
+/* Synchronises `stream`, no other one, and returns the first error that the
+ * kernels of this header have recorded on the current device since the last call
+ * (QC_ERR_BOUNDS, QC_ERR_TIMEOUT), clearing it.  The device has one such word:
+ * whoever checks gets what any caller's kernels recorded, each error once.  May be
+ * called from several threads; not while `stream` is being captured.  The first
+ * call loads a kernel, for which the driver may wait for other streams. */
 int qc_kv8_check(qc_stream stream);
 
 #ifdef __cplusplus

@@ -13,6 +13,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <mutex>
 
 #include <cuda_fp16.h>
 
@@ -30,8 +31,11 @@ constexpr int HEAD_BYTES = 16;  // a block's scales
 
 __host__ __device__ constexpr int block_bytes(int dim) { return HEAD_BYTES + 2 * BT * dim; }
 
-// First error of these kernels on this device since the last qc_kv8_check.
-__device__ int g_kv8_error;
+// First error of these kernels on this device since the last qc_kv8_check, and the one
+// that a check took away: in one step, so that none recorded meanwhile is lost.
+__device__ int g_kv8_error, g_kv8_taken;
+
+__global__ void kv8_take_error_kernel() { g_kv8_taken = atomicExch(&g_kv8_error, 0); }
 
 __device__ __forceinline__ int64_t blocks_touched(int64_t pos, int64_t cnt) {
   return cnt > 0 ? (pos + cnt - 1) / BT - pos / BT + 1 : 0;
@@ -1390,11 +1394,19 @@ extern "C" int qc_kv8_attn_decode(const qc_kv8_cache* cache, const int32_t* page
 }
 
 extern "C" int qc_kv8_check(qc_stream stream) {
-  cudaError_t e = cudaStreamSynchronize((cudaStream_t)stream);
+  static std::mutex one_at_a_time;  // g_kv8_taken is a check's until it is read
+  cudaStream_t s = (cudaStream_t)stream;
   int code = 0;
-  const int zero = 0;
-  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&code, qc::g_kv8_error, sizeof(int));
-  if (e == cudaSuccess && code) e = cudaMemcpyToSymbol(qc::g_kv8_error, &zero, sizeof(int));
+  cudaError_t e = cudaStreamSynchronize(s);
+  if (e == cudaSuccess) {
+    std::lock_guard<std::mutex> lock(one_at_a_time);
+    qc::kv8_take_error_kernel<<<1, 1, 0, s>>>();
+    e = cudaGetLastError();
+    if (e == cudaSuccess)
+      e = cudaMemcpyFromSymbolAsync(&code, qc::g_kv8_taken, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
+    const cudaError_t done = cudaStreamSynchronize(s);
+    if (e == cudaSuccess) e = done;
+  }
   if (e != cudaSuccess) return qc::refuse(QC_ERR_CUDA, "qc_kv8_check: %s", cudaGetErrorString(e));
   if (code)
     return qc::refuse(code, "qc_kv8: the device reported %s",
