@@ -13,8 +13,11 @@
 
 namespace qc {
 
-// Sets qc_last_error(NULL) and returns `code`.
+// Sets qc_last_error(NULL) and returns `code`.  The runtime keeps the last error of a
+// thread until someone takes it: left there, a launch that failed here would be found
+// by the next call's own check.
 inline int refuse(int code, const char* fmt, ...) {
+  if (code == QC_ERR_CUDA) cudaGetLastError();
   char buf[256];
   va_list ap;
   va_start(ap, fmt);
@@ -42,10 +45,7 @@ class BufferCheck {
     cudaPointerAttributes at{};
     cudaError_t e = dev_ < 0 ? cudaGetDevice(&dev_) : cudaSuccess;
     if (e == cudaSuccess) e = cudaPointerGetAttributes(&at, p);
-    if (e != cudaSuccess) {
-      cudaGetLastError();
-      return fail(QC_ERR_CUDA, name, cudaGetErrorString(e));
-    }
+    if (e != cudaSuccess) return fail(QC_ERR_CUDA, name, cudaGetErrorString(e));
     if (at.type == cudaMemoryTypeManaged) return *this;
     if (at.type != cudaMemoryTypeDevice) return fail(QC_ERR_ARG, name, "is not device memory");
     if (at.device != dev_) return fail(QC_ERR_ARG, name, "is not on the current device");

@@ -1400,8 +1400,7 @@ extern "C" int qc_kv8_check(qc_stream stream) {
   cudaError_t e = cudaStreamSynchronize(s);
   if (e == cudaSuccess) {
     std::lock_guard<std::mutex> lock(one_at_a_time);
-    qc::kv8_take_error_kernel<<<1, 1, 0, s>>>();
-    e = cudaGetLastError();
+    e = cudaLaunchKernel(qc::kv8_take_error_kernel, dim3(1), dim3(1), nullptr, 0, s);
     if (e == cudaSuccess)
       e = cudaMemcpyFromSymbolAsync(&code, qc::g_kv8_taken, sizeof(int), 0, cudaMemcpyDeviceToHost, s);
     const cudaError_t done = cudaStreamSynchronize(s);
