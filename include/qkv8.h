@@ -28,7 +28,7 @@
  * shrinks while it keeps a token.  The result depends only on which rows each
  * call wrote.
  *
- * All positions are int32, all offsets 64-bit.  A page id outside the pool, a
+ * All positions are int32 (arrays 4-byte aligned), all offsets 64-bit.  A page id outside the pool, a
  * position outside the page table's row or a row index outside the input is
  * skipped and recorded as QC_ERR_BOUNDS, which qc_kv8_check reports.
  * Calls that touch the same pages, and calls that share a workspace, must not

@@ -93,7 +93,7 @@ typedef struct qc_rope_part {
 /* Applies the rotation to n_parts groups of n_rows rows in one launch.
  * head_dim: a multiple of 8, rot_dim <= head_dim <= QC_ROPE_MAX_DIM; x, out
  * 16-byte aligned with strides multiples of 8 elements; norm_w 16-byte
- * aligned; pos_dev [n_rows] int32; n_rows 0 is a no-op.  eps >= 0 is the
+ * aligned; pos_dev [n_rows] int32, 4-byte aligned; n_rows 0 is a no-op.  eps >= 0 is the
  * norm's.  rope and parts are host pointers, read before the call returns.
  * The part's memory has to be on the current device.  No allocation; CUDA-
  * graph capturable.  QC_OK, QC_ERR_ARG or QC_ERR_CUDA (qc_last_error(NULL)). */

@@ -28,6 +28,7 @@ inline int refuse(int code, const char* fmt, ...) {
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
 // The buffers of a call, each of which a kernel launched here may follow: device
 // memory of the current device (a host pointer, or one of another device, would

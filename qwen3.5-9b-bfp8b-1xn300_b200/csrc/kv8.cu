@@ -1239,6 +1239,8 @@ int rows_call(const char* call, bool write, const qc_kv8_cache* c, const int32_t
                   (long long)k_ld, (long long)v_ld, (long long)width);
   if (!aligned16(k) || !aligned16(v))
     return refuse(QC_ERR_ARG, "%s: k and v must be 16-byte aligned", call);
+  if (!aligned4(table) || !aligned4(pos) || !aligned4(start))
+    return refuse(QC_ERR_ARG, "%s: page table, pos and row_start must be 4-byte aligned", call);
   rc = check_table(call, pt_stride, n);
   if (rc || n == 0 || rows == 0) return rc;
   rc = BufferCheck(call)
@@ -1348,6 +1350,8 @@ extern "C" int qc_kv8_attn_decode(const qc_kv8_cache* cache, const int32_t* page
   if (!qc::aligned16(q_dev) || !qc::aligned16(gate_dev) || !qc::aligned16(out_dev) ||
       !qc::aligned16(workspace))
     return qc::refuse(QC_ERR_ARG, "%s: q, gate, out and workspace must be 16-byte aligned", CALL);
+  if (!qc::aligned4(page_table_dev) || !qc::aligned4(len_dev))
+    return qc::refuse(QC_ERR_ARG, "%s: page table and len must be 4-byte aligned", CALL);
   rc = qc::check_table(CALL, pt_stride, n);
   if (rc || n == 0) return rc;
   const int64_t need = qc_kv8_attn_workspace_bytes(cache, n, n_head);

@@ -308,6 +308,7 @@ extern "C" int qc_rope_apply(const qc_rope* rope, int32_t head_dim, float eps,
     if (((uintptr_t)q.x | (uintptr_t)q.out | (uintptr_t)q.norm_w) & 15)
       return bad("x, out and norm_w must be 16-byte aligned");
   }
+  if (!qc::aligned4(pos_dev)) return bad("pos_dev must be 4-byte aligned");
   if (n_rows == 0) return QC_OK;
   qc::BufferCheck buffers(CALL);
   buffers.need("pos_dev", pos_dev);
