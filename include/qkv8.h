@@ -28,9 +28,9 @@
  * shrinks while it keeps a token.  The result depends only on which rows each
  * call wrote.
  *
- * All positions are int32 (arrays 4-byte aligned), all offsets 64-bit.  A page id outside the pool, a
- * position outside the page table's row or a row index outside the input is
- * skipped and recorded as QC_ERR_BOUNDS, which qc_kv8_check reports.
+ * All positions are int32 (arrays 4-byte aligned), all offsets 64-bit.  A page id
+ * outside the pool, a position outside the page table's row or a row index outside
+ * the input is skipped and recorded as QC_ERR_BOUNDS, which qc_kv8_check reports.
  * Calls that touch the same pages, and calls that share a workspace, must not
  * overlap on the GPU: enqueue them on one stream or order the streams (two
  * graphs that may run at once need a workspace each).

@@ -694,7 +694,8 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
   auto issue = [&]() {  // lane 0: the copy of step p into the next stage
     if (p.unit >= end) return;
     const int32_t block = p.at * GB;
-    const int32_t page = __ldg(a.table + int64_t(p.seq) * a.pt_stride + block / PAGE_BLOCKS);
+    // not by a read-only load: this kernel may be up while the table is still being written
+    const int32_t page = a.table[int64_t(p.seq) * a.pt_stride + block / PAGE_BLOCKS];
     const bool ok = page >= 0 && page < a.n_pages;
     const int32_t tokens = min(p.len - block * BT, GB * BT);
     sm.valid[w][put] = ok ? tokens : 0;
