@@ -17,7 +17,9 @@
  * pool starts at p times that; inside a page the bytes stand in the order in
  * which the attention kernel's lanes read them, so a pool is written and read
  * through the calls below.  Page ids are the caller's, for instance those that
- * qc_seq_pages gives for a sequence of a context.
+ * qc_seq_pages gives for a sequence of a context; the context knows nothing of the
+ * pool, so where it gives tokens another page (a shared page's private copy, a
+ * restored tail) the pool's bytes are the caller's to copy or to write again.
  *
  * Quantisation (qc_kv8_write).  A block's scale is the smallest power of two
  * 2^e, -126 <= e <= 120, for which every value fits (|x| <= 127 * 2^e), and
