@@ -102,8 +102,10 @@ int qc_kv8_read(const qc_kv8_cache* cache, const int32_t* page_table_dev, int32_
  * out must not overlap q, the gate or the pool.
  * workspace: at least qc_kv8_attn_workspace_bytes bytes of device memory, 16-
  * byte aligned, for this call alone while it runs; its contents do not matter.
- * Products of queries and codes are exact and sums are kept in f32; the softmax
- * weights enter the second product with 22 bits.  The result rounds to bf16 once.  It
+ * Products of queries and codes are exact (of a query value below 2^-30 of its head's
+ * largest, what is below 2^-38 of that is rounded) and sums are kept in f32; the softmax
+ * weights, with V's scales, enter the second product with 22 bits (one below 2^-10 of
+ * the largest with an error of 2^-32 of that).  The result rounds to bf16 once.  It
  * depends on the shapes and values alone: the same bits on every call.  A NaN or
  * infinity in q makes its head's row NaN, and so does a score beyond f32; finite
  * scores are right however far apart q, K and the scale are. */

@@ -431,7 +431,8 @@ __global__ void __launch_bounds__(32 * TW, WRITE ? 4 : 1) kv8_rows_kernel(const 
 // record for the four.
 //
 // Products.  S = K q on m16n8k16 f16 with f32 sums: the codes are whole numbers
-// up to 127 and the bf16 queries, scaled by a power of two, are exact in f16, so
+// up to 127 and the bf16 queries, scaled by a power of two, are exact in f16 down to
+// 2^-30 of their head's largest (below that they round, by at most 2^-38 of it), so
 // the products are exact.  Two byte permutes and two subtractions turn four
 // codes into f16: byte u under 0x64 is 1024 + u, less 1152 the code.  The row
 // order of the cache makes S, transposed by movmatrix, the operand of
@@ -440,7 +441,8 @@ __global__ void __launch_bounds__(32 * TW, WRITE ? 4 : 1) kv8_rows_kernel(const 
 // The weights of the second product carry V's scale: w = 2^(x + log2 sv - r)
 // with a running reference r of its own, so blocks of very different scales
 // keep their precision (l has no part in it).  w stands in f16, at most 2^15, and
-// w - f16(w) beside it, so that 22 bits of it count: in the product's other 4
+// w - f16(w) beside it, so that 22 bits of it count (of a w below 2^-3, which is 2^-10
+// of the largest or less, those above 2^-25): in the product's other 4
 // columns for groups of up to 4 heads, in a second product for larger ones (64 x
 // 4096 with 6 heads of 128 to a KV head 86.5 -> 87.8 us, 33 sequences of up to 8191
 // 20.0 -> 21.0).  Both references move only when a score passes them by 2^8 (m; r
@@ -747,7 +749,8 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
       top = max(top & 0xffffu, top >> 16);
       top = max(top, __shfl_xor_sync(FULL_MASK, top, 1));
       top = max(top, __shfl_xor_sync(FULL_MASK, top, 2));
-      // q / 2^e: the largest value into [2^13, 2^14), so that values 2^-37 of it stay exact.
+      // q / 2^e: the largest value into [2^13, 2^14), so that values down to 2^-30 of it stay
+      // exact: their 8 bits end at 2^-24, as f16 does.
       // The products count for scale * 2^at, one factor of which is applied before K's scale
       // and one after it, so that a score whose factors are far apart (q near 2^120, K near
       // 2^-120) leaves f32 at no step.
