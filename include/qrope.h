@@ -18,8 +18,11 @@
  * interleaved one.  Dims from rot_dim on are copied (normalised if asked).
  * Angles are formed and reduced in 64 bits for any int32 position, also a
  * negative one; the arithmetic is f32 and rounds to bf16 once, to nearest even.
- * NaN and infinity propagate within their own head: through the norm to the
- * whole head, without it to the pair they stand in.
+ * NaN and infinity stay within their own head.  Without the norm they reach the
+ * pair they stand in.  Through the norm a NaN reaches the whole head; an infinity
+ * makes the mean infinite, so that it and its pair become NaN and all other dims 0
+ * (of either sign), as the formula has it.  Finite values are normalised right
+ * however large or small they are.
  */
 #ifndef QROPE_H
 #define QROPE_H

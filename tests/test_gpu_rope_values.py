@@ -60,3 +60,29 @@ def test_norm_of_very_large_and_small_heads(qcache, dim, rot, half, power, eps):
     check(out, *reference(x, pos, list(rope.freq.inv_freq[: rot // 2]), rot, half, w, eps))
     beside = apply(qcache, rope, plain, pos, w, eps)
     assert torch.equal(out[~odd].view(torch.int16), beside[~odd].view(torch.int16))
+
+
+@pytest.mark.parametrize("half", [True, False])
+@pytest.mark.parametrize("dim,rot,at", [(64, 32, 5), (64, 32, 21), (64, 32, 50), (256, 64, 255), (40, 38, 3), (40, 38, 39)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_non_finite_values_through_the_norm(qcache, bad, dim, rot, at, half):
+    """A NaN takes its whole head; an infinity is NaN in its pair and 0 elsewhere; the
+    other heads keep their bits."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(dim + at)
+    x = torch.randn(2, 3, dim, generator=g, device="cuda").bfloat16()
+    pos = torch.tensor([5, 9], dtype=torch.int32, device="cuda")
+    w = 1 + 0.1 * torch.randn(dim, generator=g, device="cuda")
+    rope = qcache.Rope(rot, layout=qcache.ROPE_HALF if half else qcache.ROPE_INTERLEAVED)
+    clean = apply(qcache, rope, x, pos, w, 1e-6)
+    x[1, 1, at] = bad
+    got = apply(qcache, rope, x, pos, w, 1e-6)
+    pair = {at} if at >= rot else {at, (at + rot // 2) % rot if half else at ^ 1}
+    for d in range(dim):
+        y = float(got[1, 1, d])
+        if bad != bad or d in pair:
+            assert y != y, (d, y)
+        else:
+            assert y == 0, (d, y)
+    got[1, 1] = clean[1, 1]
+    assert torch.equal(got.view(torch.int16), clean.view(torch.int16))
