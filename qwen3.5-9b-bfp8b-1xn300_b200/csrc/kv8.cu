@@ -448,10 +448,10 @@ __global__ void __launch_bounds__(32 * TW, WRITE ? 4 : 1) kv8_rows_kernel(const 
 // 20.0 -> 21.0).  Both references move only when a score passes them by 2^8 (m; r
 // starts 2^7 under its largest and moves at 2^15), so most blocks rescale nothing.
 //
-// Bound by memory: 64 sequences of 4096 with 4 heads of 256 (538 MB) 88 us, 6.1 TB/s,
-// 0.93 of the measured copy rate, the merge included.  A block costs a warp 32
-// products of 8 cycles and some 550 other instructions, a third of what the SM could
-// issue meanwhile.  mma.sync and not tcgen05: with 1 to 8 query rows the tensor pipe
+// Bound by memory: 64 sequences of 4096 with 4 heads of 256 (538 MB) 87 us, 6.2 TB/s,
+// 0.95 of the measured copy rate, the merge included.  A block costs a warp 32
+// products of 8 cycles (48 for groups above 4) and some 590 other instructions, half of
+// what the SM could issue meanwhile.  mma.sync and not tcgen05: with 1 to 8 query rows the tensor pipe
 // has little to do, and the codes pass through registers on the way to f16 anyway.
 
 struct Kv8AttnArgs {
@@ -1042,6 +1042,8 @@ constexpr int MERGE_CTAS = 592;
 
 template <int D, int LOG_CHUNK, int LOG_HG>
 __global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnArgs a) {
+  // a thread's records in flight with the heads; 2, 5 and 8 of them (us): 1 x 1024 9.2, 8.8,
+  // 9.2; 16 x 4096 27.5, 27.3, 28.7; 1 x 131072 with one KV head of 256 20.3, 18.8, 19.0
   constexpr int AHEAD = 5;
   __shared__ float4 part[256];
   __shared__ float ref[LOG_HG == 0 ? MAX_WARPS : 1];  // one head: the records' r

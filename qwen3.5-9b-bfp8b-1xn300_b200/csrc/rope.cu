@@ -6,9 +6,10 @@
 // dims) or 8 dims (the rest), so it works out its four cosines and sines once,
 // keeps them in registers over all heads that it takes, and no lane needs
 // another's values except for the norm's sum.  32768 rows of 40 heads of 128 (671
-// MB) take 112.7 us, 5.96 TB/s, 0.91 of the measured copy rate; an earlier form, a
+// MB) take 113 us, 5.94 TB/s, 0.90 of the measured copy rate; an earlier form, a
 // CTA per row with the pairs exchanged through shared memory, took 416 us: too few
-// loads in flight behind its barriers.
+// loads in flight behind its barriers.  With the norm an SM issues an instruction in
+// two cycles of three (2048 rows of 20 heads of 256: 11.8 us, 6.4 by its bytes).
 #include <algorithm>
 #include <cmath>
 #include <cstring>
@@ -51,8 +52,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 // 8 dims; all lanes of the warp call it.  Where the squares leave f32 (values beyond
 // 1.8e19, or all below 3e-14 with as small an eps) y is first brought to about 1 by a
 // power of two, exactly but for what is 2^-126 of the head's largest value.  The vote on
-// that costs 2048 rows of 20 heads of 256 0.6 of 11.8 us; one vote for four heads, or
-// a loop of their own for such heads, costs as much or more, in registers.
+// that costs 0.6 us of the 11.8 of 2048 rows of 20 heads of 256; one vote for four heads,
+// or a loop of their own for such heads, costs as much or more, in registers.
 __device__ __forceinline__ float norm_factor(const RopeArgs& a, float (&y)[8]) {
   const auto mean = [&](float eps) {
     float ss = 0.0f;
@@ -346,11 +347,11 @@ extern "C" int qc_rope_apply(const qc_rope* rope, int32_t head_dim, float eps,
       most = std::max(most, int32_t(parts[p].n_heads));
     }
     // A group takes as many of its row's heads as leave WANT threads (two waves of
-    // every SM), as each group works out the row's angles again: 2048 rows of 20
-    // normalised heads of 256 take 10.9 us so, 16.1 with half as many threads.  With
-    // fewer than FEW threads one head to a group is faster, the others' loads and
-    // arithmetic being latency alone: 8 rows 2.0 against 3.0 us, 64 rows 2.8 and
-    // 3.1, 128 rows 3.6 and 3.3.
+    // each of a B200's 148 SMs), as each group works out the row's angles again: 2048 and
+    // 4096 rows of 20 normalised heads of 256 take 11.8 and 20.6 us so, 12.7 and 25.9 with
+    // half as many threads.  With fewer than FEW threads one head to a group is faster,
+    // the others' loads and arithmetic being latency alone: 8 rows 1.9 against 3.2 us, 64
+    // rows 2.7 and 3.3, 128 rows 3.2 and 3.6; 1024 rows 10.0 and 6.6.
     auto slices = [&](int32_t chunk) {
       int32_t n = 0;
       for (int p = 0; p < n_parts; ++p) n += a.slices[p] = (int32_t(parts[p].n_heads) + chunk - 1) / chunk;
