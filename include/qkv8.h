@@ -107,8 +107,8 @@ int qc_kv8_read(const qc_kv8_cache* cache, const int32_t* page_table_dev, int32_
  * weights, with V's scales, enter the second product with 22 bits (one below 2^-10 of
  * the largest with an error of 2^-32 of that).  The result rounds to bf16 once.  It
  * depends on the shapes and values alone: the same bits on every call.  A NaN or
- * infinity in q makes its head's row NaN, and so does a score beyond f32; finite
- * scores are right however far apart q, K and the scale are. */
+ * infinity in q makes its head's row NaN, and scores beyond f32 may.  Scores up to
+ * 2^100 are formed without leaving f32 however far apart q, K and the scale are. */
 int64_t qc_kv8_attn_workspace_bytes(const qc_kv8_cache* cache, int32_t n, int32_t n_head);
 int qc_kv8_attn_decode(const qc_kv8_cache* cache, const int32_t* page_table_dev,
                        int32_t pt_stride, const int32_t* len_dev, int32_t n, int32_t n_head,

@@ -628,8 +628,9 @@ __global__ void __launch_bounds__(32 * AW, ctas_per_sm(D)) kv8_attn_kernel(const
   const auto share = [&]() {
     per = max(quotient(total + warps - 1, warps), int64_t(1));
     // ranges side by side are one CTA's, so that it can join them; when there is at most
-    // one step for each warp and few for a pair (1 x 1024: 8.5 us, joined 9.1; with 313
-    // steps in one pair 8.3 and 7.3) they go to different SMs
+    // one step for each warp and few for a pair they go to different SMs: 4 heads of 256, 64
+    // steps each, 8.5 us so and 9.3 joined, 128 steps 9.2 and 9.5, 160 the same, 200 10.0 and
+    // 9.6 (one head alone turns at some 40 steps, 0.2 to 0.8 us apart up to 128)
     spread = total <= warps && total <= int64_t(128) * a.n * a.kv_heads;
   };
   const auto range_of = [&](int x) { return spread ? x * int(gridDim.x) + int(blockIdx.x) : int(blockIdx.x) * AW + x; };
