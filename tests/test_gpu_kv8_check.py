@@ -58,7 +58,7 @@ def test_an_error_is_reported_to_one_of_several_threads(qcache):
     start, end = threading.Barrier(threads + 1), threading.Barrier(threads + 1)
     seen = [[] for _ in range(rounds)]
 
-    def checker(stream):
+    def ask(stream):
         for r in range(rounds):
             start.wait()
             try:
@@ -67,7 +67,7 @@ def test_an_error_is_reported_to_one_of_several_threads(qcache):
                 seen[r].append(e.code)
             end.wait()
 
-    ts = [threading.Thread(target=checker, args=(s,), daemon=True) for s in streams]
+    ts = [threading.Thread(target=ask, args=(s,), daemon=True) for s in streams]
     for t in ts:
         t.start()
     for r in range(rounds):
